@@ -376,6 +376,105 @@ int pkv_paged_prefill_rows(void* out, int out_dtype, int64_t out_stride_tok, int
                            void* stream);
 
 /*
+ * Attention with modified scores (no counterpart in the reference, whose models cap no score and
+ * mask causally only). The arguments after num_rows of the two calls below:
+ *   softcap (0: none; else 1e-30 .. 1e30): s = softcap * tanh(scale * q . k / softcap);
+ *   alibi_slopes (fp32 [num_heads], or NULL): s -= alibi_slopes[h] * |query's position - key's|,
+ *     after the cap; a decode query sits at context_lens[b] - 1, query i of a chunk of q_c tokens
+ *     at n_c - q_c + i. Slopes are finite;
+ *   key_ranges (int32 pairs [first, last), row stride range_stride elements, or NULL): the query in
+ *     row r of q attends to keys first <= p < last of its context (cut to [0, n)) and to no others,
+ *     instead of the causal limit: sliding windows, documents, prefixes that see themselves both
+ *     ways. One pair per row of q (rows[b] picks q's row and its pair). An empty range gives 0.
+ *     Keys outside a row's range do not reach it, whatever they hold, NaN and infinities included;
+ *   lse (fp32 [batch or tokens, num_heads], contiguous, or NULL): log2 normalisers as in
+ *     pkv_paged_decode_ex, of the modified scores, in the order of the sequences (of the step's
+ *     query tokens); -inf where no key was seen. Rows that are skipped keep what they hold.
+ * Everything else is pkv_paged_decode_rows (rows NULL: row b of q, num_rows = batch) and
+ * pkv_paged_prefill_rows (rows NULL: row t); scale must be positive and finite. num_workgroups 0
+ * takes pkv_decode_mod_default_workgroups() ranges, whose workspace the caller passes (0: none).
+ */
+int pkv_paged_decode_mod(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride_h,
+                         const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                         const void* k_cache, const void* v_cache, int kv_dtype,
+                         int64_t kv_stride_slot, int64_t kv_stride_head, int64_t num_slots,
+                         const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+                         const int32_t* context_lens, int32_t batch, int32_t num_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         float scale, int32_t num_workgroups, void* workspace,
+                         int64_t workspace_bytes, const int64_t* rows, int64_t num_rows,
+                         float softcap, const float* alibi_slopes, const int32_t* key_ranges,
+                         int64_t range_stride, float* lse, void* stream);
+
+int32_t pkv_decode_mod_default_workgroups(int kv_dtype, int32_t head_dim, int32_t num_heads,
+                                          int32_t num_kv_heads, int32_t batch, int32_t max_blocks,
+                                          int32_t block_size);
+
+int pkv_paged_prefill_mod(void* out, int out_dtype, int64_t out_stride_tok, int64_t out_stride_h,
+                          const void* q, int64_t q_stride_tok, int64_t q_stride_h,
+                          const void* k_cache, const void* v_cache, int kv_dtype,
+                          int64_t kv_stride_slot, int64_t kv_stride_head, int64_t num_slots,
+                          const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+                          const int32_t* context_lens, const int32_t* cu_seqlens_q, int32_t n_chunks,
+                          int32_t max_query_len, int32_t num_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t block_size, float scale, void* workspace,
+                          int64_t workspace_bytes, const int64_t* rows, int64_t rows_len,
+                          int64_t num_rows, float softcap, const float* alibi_slopes,
+                          const int32_t* key_ranges, int64_t range_stride, float* lse, void* stream);
+
+/*
+ * Accumulated attention weights (no counterpart in the reference, which evicts no token). For
+ * chunk c with query tokens cu_seqlens_q[c] .. cu_seqlens_q[c+1]-1 of q, last in its context of n_c
+ * tokens (cu_seqlens_q NULL: one query per chunk, row c), and every p < n_c:
+ *   w[p] = decay * w[p] + sum over its queries t and all heads h that see p of
+ *          2^(s(t, h, p) - lse[t, h]),
+ * s in log2 units, i.e. the softmax weights of the attention call that wrote lse (fp32 [tokens,
+ * num_heads], contiguous) with the same softcap, alibi_slopes and key_ranges (as above, one range
+ * per row of q; NULL: causal). A query whose lse is -inf gives nothing. w is row weight_rows[c]
+ * (int64 [n_chunks]; NULL: c) of weights (fp32, num_weight_rows rows, row stride weight_stride,
+ * at least max_blocks * block_size long); a chunk whose row lies outside is skipped; chunks that
+ * name one row leave one of the results. decay 0: what w held is not read. Positions from n_c on
+ * stay as they are. Sums are fp32, in a fixed order; out-of-range block ids hold no key.
+ */
+int pkv_attention_weights(float* weights, int64_t weight_stride, int64_t num_weight_rows,
+                          const int64_t* weight_rows, float decay, const void* q,
+                          int64_t q_stride_tok, int64_t q_stride_h, const void* k_cache,
+                          int kv_dtype, int64_t kv_stride_slot, int64_t kv_stride_head,
+                          int64_t num_slots, const int32_t* block_tables, int64_t table_stride,
+                          int32_t max_blocks, const int32_t* context_lens,
+                          const int32_t* cu_seqlens_q, int32_t n_chunks, const float* lse,
+                          int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t block_size, float scale, float softcap,
+                          const float* alibi_slopes, const int32_t* key_ranges,
+                          int64_t range_stride, void* stream);
+
+/*
+ * Eviction by accumulated weight (no counterpart in the reference). In every layer l, sequence b of
+ * n = clamp(context_lens[b], 0, max_blocks * block_size) > keep tokens keeps its last `recent`
+ * ones and, of the others, the keep - recent with the largest w[p] (ties: the lowest positions; a
+ * NaN counts as the smallest), and loses the rest: the kept tokens' K and V rows move, in their
+ * order, to the slots of positions 0 .. keep - 1, their weights likewise, and w[keep .. n-1]
+ * becomes 0. Slots of positions from keep on keep what they hold. new_lens[b] = min(n, keep).
+ * w is row weight_rows[b] (NULL: b) of layer l's weights; a sequence whose row lies outside
+ * [0, num_weight_rows) is left alone (new_lens[b] = context_lens[b]).
+ * Pools: per layer num_slots rows of row_bytes contiguous bytes (a multiple of 16), layers
+ * layer_stride_bytes apart. The blocks of an evicted sequence must be its own (copy-on-write
+ * first: rows move in place), no block twice in its table, weight rows distinct; tokens whose
+ * block id lies outside the pool are not moved. workspace: pkv_evict_workspace_bytes() bytes,
+ * 8-byte aligned, any contents. new_lens may be context_lens.
+ */
+int64_t pkv_evict_workspace_bytes(int32_t layers, int32_t batch, int32_t max_blocks,
+                                  int32_t block_size, int32_t keep);
+
+int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride_bytes, int32_t layers,
+              int64_t row_bytes, int64_t num_slots, float* weights, int64_t weight_stride_layer,
+              int64_t weight_stride_row, int64_t num_weight_rows, const int64_t* weight_rows,
+              const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+              int32_t block_size, const int32_t* context_lens, int32_t batch, int32_t keep,
+              int32_t recent, int32_t* new_lens, void* workspace, int64_t workspace_bytes,
+              void* stream);
+
+/*
  * Fused element-wise kernels (csrc/fused.hip). Replace the reference's Triton kernels of
  * engine/kernels/fused.py:47-131 (rms_norm, rope_, silu_mul), with the same contract:
  * every result is bitwise identical to the PyTorch ops they stand for.

@@ -2,10 +2,10 @@
 
     python inference-engine_amd/csrc/build.py
 
-compiles csrc/kv_ops.hip, csrc/decode.hip, csrc/prefill.hip, csrc/cascade.hip (sharing
+compiles csrc/kv_ops.hip, csrc/decode.hip, csrc/prefill.hip, csrc/cascade.hip,
+csrc/decode_mod.hip, csrc/prefill_mod.hip, csrc/weights.hip and csrc/evict.hip (sharing
 csrc/common.h and the kernel headers) and csrc/fused.hip with hipcc for gfx950 into
-lib/libpaged_kv.so (next to the engine
-package). The library links libamdhip64.so.7;
+lib/libpaged_kv.so (next to the engine package). The library links libamdhip64.so.7;
 loaded after ``import torch`` it binds to the HIP runtime torch already loaded (same
 SONAME), so torch's streams and device pointers are valid inside it.
 """
@@ -24,7 +24,9 @@ PKG_ROOT = os.path.dirname(HERE)
 REPO = os.path.dirname(PKG_ROOT)
 LIB_DIR = os.path.join(PKG_ROOT, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpaged_kv.so")
-SOURCES = [os.path.join(HERE, f) for f in ("kv_ops.hip", "decode.hip", "prefill.hip", "cascade.hip", "fused.hip")]
+SOURCES = [os.path.join(HERE, f) for f in (
+    "kv_ops.hip", "decode.hip", "decode_mod.hip", "prefill.hip", "prefill_mod.hip", "cascade.hip",
+    "weights.hip", "evict.hip", "fused.hip")]  # fmt: skip
 INCLUDE = os.path.join(REPO, "include")
 
 HIPCC_FLAGS = [

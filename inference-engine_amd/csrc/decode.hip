@@ -4,7 +4,7 @@
 // combine (kernels in decode_kernels.h).
 
 #include "cascade.h"
-#include "decode_kernels.h"
+#include "decode_dispatch.h"
 
 #include <algorithm>
 #include <mutex>
@@ -49,96 +49,12 @@ DecodeWs decode_ws(int32_t num_wg, int32_t batch, int32_t nh, int32_t hd, bool c
   return w;
 }
 
-// The MFMA kernel serves 16-bit K/V at head_dim 64 and 128; every other shape uses the
-// generic stream kernel.
-template <int DT, int HD> constexpr bool use_mfma() {
-  return DT != PKV_F32 && (HD == 128 || HD == 64) && PKV_DECODE_USE_MFMA;
-}
-
-// Run f.run<DT, HD, GPW>() for the runtime (dtype, head_dim, heads per wave).
-template <int DT, int HD, class F> hipError_t by_gpw(int gpw, const F& f) {
-  switch (gpw) {
-    case 1: return f.template run<DT, HD, 1>();
-    case 2: return f.template run<DT, HD, 2>();
-    case 3: return f.template run<DT, HD, 3>();
-    case 4: return f.template run<DT, HD, 4>();
-    default:  // only planned where the MFMA kernel serves the shape (plan_decode)
-      if constexpr (use_mfma<DT, HD>()) return f.template run<DT, HD, kWideHeads>();
-      else return hipErrorInvalidValue;
-  }
-}
-template <int DT, class F> hipError_t by_hd(int hd, int gpw, const F& f) {
-  switch (hd) {
-    case 16: return by_gpw<DT, 16>(gpw, f);
-    case 32: return by_gpw<DT, 32>(gpw, f);
-    case 64: return by_gpw<DT, 64>(gpw, f);
-    case 128: return by_gpw<DT, 128>(gpw, f);
-    default: return by_gpw<DT, 256>(gpw, f);
-  }
-}
-template <class F> hipError_t by_dtype(int dt, int hd, int gpw, const F& f) {
-  switch (dt) {
-    case PKV_F32: return by_hd<PKV_F32>(hd, gpw, f);
-    case PKV_F16: return by_hd<PKV_F16>(hd, gpw, f);
-    default: return by_hd<PKV_BF16>(hd, gpw, f);
-  }
-}
-
 template <int DT, int HD, int GPW> const void* decode_kernel() {
   if constexpr (use_mfma<DT, HD>())
     return reinterpret_cast<const void*>(
         &paged_decode_mfma_kernel<DT, stream_gpw<HD, GPW>(), true, HD, false>);
   else
     return reinterpret_cast<const void*>(&paged_decode_stream_kernel<DT, HD, GPW, false>);
-}
-
-// Dynamic LDS of the stream pass's workgroups of wpg waves.
-template <int DT, int HD, int GPW> constexpr unsigned stream_lds(int wpg) {
-  return use_mfma<DT, HD>() && pv_mfma<HD, GPW>() ? (unsigned)(wpg * kVSlotBytes) : 0u;
-}
-
-// Waves the combine gives each (sequence, head) pair: there are as many ranges for any
-// batch, so with few pairs each has many records, and one wave folds them in dependent
-// trips of a few rows each. Whole decode calls with 1 / 2 / 4 / 8 / 16 waves per pair (us):
-//   32 pairs (1 sequence of 20,011 tokens, hd 128)  45.2 / 34.8 / 28.7 / 26.2 / 25.7
-//   64 pairs (2 sequences of 3,000-9,000)           33.7 / 26.8 / 21.9 / 20.6 / 20.5
-//   128 pairs (4 such)                              32.8 / 29.3 / 27.1 / 26.2 / 26.8
-//   256 pairs (8 such)                              42.6 / 41.1 / 39.6 / 39.8 / 40.3
-//   512 pairs (16 of 1,000-4,000)                   35.0 / 34.2 / 34.1 / 34.4 / 38.0
-//   1,024 pairs (64 of 200-3,000, 16 heads)         71.3 / 71.4 / 72.1 / 74.6 / 77.9
-//   1,024 pairs (32 of 128-32,768, log)            106.9 / 105.7 / 105.0 / 106.5 / 110.1
-//   1,536 pairs (64 of 1,024-4,096, 24 heads)      109.8 / 110.0 / 111.6 / 115.0 / 119.8
-//   768 pairs (24 of 3,000-9,000, 24 heads)        103.4 / 101.8 / 104.2 / 105.3 / 112.0
-//   1,024 pairs (32 of 2,060-2,200)                 56.9 / 54.5 / 56.1 / 57.2 / 64.4
-//   32 pairs, hd 256 (1 of 20,011)                  65.6 / 54.0 / 47.0 / 44.4 / 44.4
-//   8 pairs, hd 256 (1 of 9,000, 8 heads)          122.2 / 74.6 / 43.8 / 34.0 / 30.3
-// (Two libraries in turn on the same buffers, hd 128: four waves up to 1,024 pairs gain 0.4-0.9%
-// where a few long sequences have most of the ranges, 32 or 24 of 128-32,768, and lose 1-2% where
-// lengths are even: 45.3 against 45.9 us for 64 of 200-3,000, 55.9 against 56.6 for 32 of
-// 2,060-2,200.)
-int combine_waves(const DecodeArgs& a) {
-  const int pairs = a.batch * a.nh;
-  if (pairs <= 64) return 16;
-  if (pairs <= 256) return 8;
-  if (pairs <= 512) return 4;
-  return pairs <= PKV_DECODE_COMBINE_SPLIT_PAIRS ? 2 : 1;
-}
-template <int DT, int HD, int SP, bool WT, bool ROWS>
-void launch_combine_sp(const DecodeArgs& a, hipStream_t st) {
-  constexpr int WG = SP > 4 ? SP : 4;  // waves per workgroup
-  const int pairs = a.batch * a.nh;
-  hipLaunchKernelGGL((paged_decode_combine_kernel<DT, HD, SP, WT, ROWS>),
-                     dim3((unsigned)((pairs + WG / SP - 1) / (WG / SP))), dim3(kWave * WG), 0, st, a);
-}
-template <int DT, int HD, bool WT, bool ROWS>
-void launch_combine(const DecodeArgs& a, hipStream_t st) {
-  switch (combine_waves(a)) {
-    case 16: return launch_combine_sp<DT, HD, 16, WT, ROWS>(a, st);
-    case 8: return launch_combine_sp<DT, HD, 8, WT, ROWS>(a, st);
-    case 4: return launch_combine_sp<DT, HD, 4, WT, ROWS>(a, st);
-    case 2: return launch_combine_sp<DT, HD, 2, WT, ROWS>(a, st);
-    default: return launch_combine_sp<DT, HD, 1, WT, ROWS>(a, st);
-  }
 }
 
 struct LaunchDecode {
@@ -294,11 +210,16 @@ int device_cus(int* cus) {
 }
 
 // Workgroups of a plan that the current device holds at once (see pkv_decode_workgroups).
-int32_t plan_workgroups(const DecodePlan& p, int kv_dtype, int head_dim) {
+int32_t plan_workgroups(const DecodePlan& p, int kv_dtype, int head_dim, bool mod = false) {
   int dev = 0, cus = 0, per_cu = 0, tile = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
   if (e == hipSuccess) e = by_dtype(kv_dtype, head_dim, p.gpw, QueryDecode{p.wpg, &tile, &per_cu});
+  if (e == hipSuccess && mod) {  // no more than without: scratch sized for that serves both
+    int n = 0;
+    e = decode_mod_per_cu(kv_dtype, head_dim, p.gpw, p.wpg, &n);
+    per_cu = std::min(per_cu, n);
+  }
   if (e != hipSuccess) return PKV_E_HIP;
   const int g = cus * (per_cu < 1 ? 1 : per_cu) / p.ygrid;
   return g < 1 ? 1 : g;
@@ -315,8 +236,9 @@ int32_t plan_workgroups(const DecodePlan& p, int kv_dtype, int head_dim) {
 //   * up to there, at least gpw / 4, down to 64 ranges: 128 / 8, one sequence of 2,500, 256 / 128
 //     / 64 21.7 / 18.6 / 17.5 (18.2 in waves of 4 heads); of 8,000, 256 / 128 / 64 27.1 / 24.2 /
 //     27.2; 64 / 8, of 8,000, 256 / 128 21.6 / 20.7.
-int32_t default_ranges(const DecodePlan& p, int kv_dtype, int head_dim, int batch, int64_t max_tokens) {
-  const int32_t full = plan_workgroups(p, kv_dtype, head_dim);
+int32_t default_ranges(const DecodePlan& p, int kv_dtype, int head_dim, int batch, int64_t max_tokens,
+                       bool mod = false) {
+  const int32_t full = plan_workgroups(p, kv_dtype, head_dim, mod);
   if (p.gpw <= 4 || full < 1) return full;
   int cus = 0;
   const int st = device_cus(&cus);
@@ -421,7 +343,8 @@ int decode_ex(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride
               const float* prefix_out, const float* prefix_lse,
               const int32_t* prefix_row, int32_t prefix_parts,
               int64_t prefix_stride, void* stream,
-              const CascadeLaunch* one, bool check_only, const int64_t* rows, int64_t num_rows) {
+              const CascadeLaunch* one, bool check_only, const int64_t* rows, int64_t num_rows,
+              const ScoreMod* mod) {
   const int bad = check_decode_shape(kv_dtype, head_dim, num_heads, num_kv_heads);
   if (bad) return bad;
   const bool cascade = prefix_row != nullptr && prefix_parts > 0;
@@ -448,7 +371,7 @@ int decode_ex(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride
     int split_gpw = 0;
     const int st = choose_split(kv_dtype, head_dim, batch, num_heads, num_kv_heads, max_blocks,
                                 (int64_t)max_blocks * block_size,
-                                cascade || first_block || lse, &split_gpw);
+                                cascade || first_block || (lse && !mod), &split_gpw);
     if (st) return st;
     split = split_gpw > 0;
     if (split) {
@@ -459,7 +382,7 @@ int decode_ex(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride
       // pkv_decode_workgroups).
       num_workgroups = cascade ? plan_workgroups(p, kv_dtype, head_dim)
                                : default_ranges(p, kv_dtype, head_dim, batch,
-                                                (int64_t)max_blocks * block_size);
+                                                (int64_t)max_blocks * block_size, mod != nullptr);
       if (num_workgroups < 1) return num_workgroups < 0 ? num_workgroups : PKV_E_HIP;
     }
   }
@@ -509,6 +432,7 @@ int decode_ex(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride
   a.fin_f32 = 0;
   a.rows = rows;
   a.num_rows = num_rows;
+  a.mod = mod ? *mod : ScoreMod{0.f, 0.f, nullptr, nullptr, 0};
   a.desc = nullptr;
   a.ws_acc = nullptr;
   a.ws_ml = nullptr;
@@ -516,6 +440,7 @@ int decode_ex(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride
   if (split) {
     if (check_only) return 0;
     a.num_wg = a.full_wg = a.slots = 1;
+    if (mod) return (int)launch_decode_mod(a, kv_dtype, head_dim, kSplitWaves, num_kv_heads * p.nsub, true, st);
     return (int)by_dtype(kv_dtype, head_dim, p.gpw,
                          LaunchSplit{&a, num_kv_heads * p.nsub, st});
   }
@@ -560,6 +485,7 @@ int decode_ex(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride
     }
   }
   if (check_only) return 0;
+  if (mod) return (int)launch_decode_mod(a, kv_dtype, head_dim, p.wpg, p.ygrid, false, st);
   return (int)by_dtype(kv_dtype, head_dim, p.gpw, LaunchDecode{&a, p.wpg, p.ygrid, st, one});
 }
 
@@ -618,6 +544,21 @@ int32_t pkv_decode_default_workgroups(int kv_dtype, int32_t head_dim, int32_t nu
                         batch, (int64_t)max_blocks * block_size);
 }
 
+int32_t pkv_decode_mod_default_workgroups(int kv_dtype, int32_t head_dim, int32_t num_heads,
+                                          int32_t num_kv_heads, int32_t batch, int32_t max_blocks,
+                                          int32_t block_size) {
+  const int bad = check_decode_shape(kv_dtype, head_dim, num_heads, num_kv_heads);
+  if (bad) return bad;
+  if (batch < 0 || max_blocks < 0 || block_size <= 0) return PKV_E_SHAPE;
+  int split_gpw = 0;
+  const int st = choose_split(kv_dtype, head_dim, batch, num_heads, num_kv_heads, max_blocks,
+                              (int64_t)max_blocks * block_size, false, &split_gpw);
+  if (st) return st;
+  if (split_gpw) return 0;
+  return default_ranges(plan_decode(kv_dtype, head_dim, num_heads, num_kv_heads), kv_dtype, head_dim,
+                        batch, (int64_t)max_blocks * block_size, true);
+}
+
 int64_t pkv_decode_workspace_bytes(int32_t num_workgroups, int32_t batch, int32_t num_heads,
                                    int32_t head_dim) {
   return decode_ws(num_workgroups, batch, num_heads, head_dim, false).total;
@@ -661,6 +602,29 @@ int pkv_paged_decode_rows(void* out, int out_dtype, int64_t out_stride_b, int64_
                    head_dim, block_size, scale, num_workgroups, workspace, workspace_bytes,
                    nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, stream, nullptr, false,
                    rows, num_rows);
+}
+
+int pkv_paged_decode_mod(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride_h,
+                         const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                         const void* k_cache, const void* v_cache, int kv_dtype,
+                         int64_t kv_stride_slot, int64_t kv_stride_head, int64_t num_slots,
+                         const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+                         const int32_t* context_lens, int32_t batch, int32_t num_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         float scale, int32_t num_workgroups, void* workspace,
+                         int64_t workspace_bytes, const int64_t* rows, int64_t num_rows,
+                         float softcap, const float* alibi_slopes, const int32_t* key_ranges,
+                         int64_t range_stride, float* lse, void* stream) {
+  ScoreMod mod;
+  const int bad = score_mod(&mod, softcap, alibi_slopes, key_ranges, range_stride);
+  if (bad) return bad;
+  if (!(scale > 0.f && scale < INFINITY)) return PKV_E_SHAPE;
+  return decode_ex(out, out_dtype, out_stride_b, out_stride_h, q, q_stride_b, q_stride_h, k_cache,
+                   v_cache, kv_dtype, kv_stride_slot, kv_stride_head, num_slots, block_tables,
+                   table_stride, max_blocks, context_lens, batch, num_heads, num_kv_heads,
+                   head_dim, block_size, scale, num_workgroups, workspace, workspace_bytes,
+                   nullptr, lse, nullptr, nullptr, nullptr, 0, 0, stream, nullptr, false,
+                   rows, num_rows, &mod);
 }
 
 int pkv_paged_decode_ex(void* out, int out_dtype, int64_t out_stride_b, int64_t out_stride_h,

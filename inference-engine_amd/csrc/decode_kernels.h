@@ -4,7 +4,7 @@
 
 #pragma once
 
-#include "common.h"
+#include "score_mod.h"
 
 namespace pkv {
 
@@ -55,6 +55,7 @@ struct DecodeArgs {
   // from the end, and a sequence whose row lies outside writes nothing.
   const int64_t* rows;
   int64_t num_rows;
+  ScoreMod mod;  // read by the kernels instantiated with MOD
 };
 
 }  // namespace pkv
@@ -97,8 +98,28 @@ template <int DT, int HD> struct DecodeShape {
 };
 
 
-// Table column sequence b starts from (a shared prefix handled elsewhere is skipped).
+__device__ __forceinline__ int64_t seq_row(const DecodeArgs& a, int b);
+
+// MOD: the keys [lo, hi) that sequence b's query sees, lo < hi, or lo = hi = 0.
+struct KeySpan {
+  int lo, hi;
+};
+__device__ __forceinline__ KeySpan key_span(const DecodeArgs& a, int b) {
+  const int cap = a.max_blocks * a.bs;
+  const int n = min(max(a.ctx[b], 0), cap);
+  if (!a.mod.ranges) return {0, n};
+  const int64_t r = seq_row(a, b);
+  if (r < 0) return {0, 0};
+  const int lo = max(a.mod.ranges[r * a.mod.range_stride], 0);
+  const int hi = min(a.mod.ranges[r * a.mod.range_stride + 1], n);
+  return lo < hi ? KeySpan{lo, hi} : KeySpan{0, 0};
+}
+
+// Table column sequence b starts from (a shared prefix handled elsewhere, or keys before its
+// range, are skipped).
+template <bool MOD = false>
 __device__ __forceinline__ int first_blk(const DecodeArgs& a, int b) {
+  if constexpr (MOD) return a.mod.ranges ? key_span(a, b).lo / a.bs : 0;
   if (!a.first_block) return 0;
   const int f = a.first_block[b];
   return f < 0 ? 0 : (f > a.max_blocks ? a.max_blocks : f);
@@ -128,8 +149,13 @@ __device__ __forceinline__ WholeDst whole_dst(const DecodeArgs& a, int pre_b) {
 }
 
 // Tokens sequence b attends to, clamped: 0 <= n <= (max_blocks - first) * block_size.
-// They are positions first * block_size + p, p < n.
+// They are positions first * block_size + p, p < n (MOD: from the range's first key on).
+template <bool MOD = false>
 __device__ __forceinline__ int clamped_ctx(const DecodeArgs& a, int b) {
+  if constexpr (MOD) {
+    const KeySpan s = key_span(a, b);
+    return s.hi - s.lo / a.bs * a.bs;
+  }
   const int fb = first_blk(a, b);
   const int n = a.ctx[b] - fb * a.bs;
   const int cap = (a.max_blocks - fb) * a.bs;
@@ -198,12 +224,13 @@ __device__ __forceinline__ int units_of(const DecodeArgs& a, int n) {
 // Wave-wide walk over the unit prefix sums. With target >= 0 returns the sequence b
 // that owns unit `target` and its first unit in *ustart; with target < 0 (or past the
 // end) returns batch and the total unit count in *ustart. Call from whole waves.
+template <bool MOD = false>
 __device__ int find_unit(const DecodeArgs& a, int64_t target, int64_t* ustart) {
   const int lane = threadIdx.x & (kWave - 1);
   int64_t base = 0;
   for (int c0 = 0; c0 < a.batch; c0 += kWave) {
     const int bb = c0 + lane;
-    const int cnt = bb < a.batch ? units_of(a, clamped_ctx(a, bb)) : 0;
+    const int cnt = bb < a.batch ? units_of(a, clamped_ctx<MOD>(a, bb)) : 0;
     int incl = cnt;
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
@@ -237,11 +264,12 @@ __device__ __forceinline__ int64_t range_start(const DecodeArgs& a, int64_t w, i
 // *ub); returns batch when the range is empty. A batch that fits one wave is scanned
 // once (the lengths' prefix sums give both the total and the owner); larger batches
 // take two passes of find_unit. Call from whole waves.
+template <bool MOD = false>
 __device__ int locate_range(const DecodeArgs& a, int w, int64_t* total, int64_t* rs,
                             int64_t* re, int64_t* ub) {
   if (a.batch <= kWave) {
     const int lane = threadIdx.x & (kWave - 1);
-    const int cnt = lane < a.batch ? units_of(a, clamped_ctx(a, lane)) : 0;
+    const int cnt = lane < a.batch ? units_of(a, clamped_ctx<MOD>(a, lane)) : 0;
     int incl = cnt;
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
@@ -257,11 +285,11 @@ __device__ int locate_range(const DecodeArgs& a, int w, int64_t* total, int64_t*
     *ub = __shfl(incl - cnt, l);
     return l;
   }
-  find_unit(a, -1, total);
+  find_unit<MOD>(a, -1, total);
   *rs = range_start(a, w, *total);
   *re = range_start(a, w + 1, *total);
   if (*rs >= *re) return a.batch;
-  return find_unit(a, *rs, ub);
+  return find_unit<MOD>(a, *rs, ub);
 }
 // The range holding unit u: the largest w with range_start(w) <= u. The largest slot s
 // with s * units / slots <= u is ((u + 1) * slots - 1) / units; w is the range that
@@ -300,6 +328,7 @@ struct BatchLds {
 };
 // Fill s (whole workgroup; blockDim.x <= 64 * PKV_DECODE_WAVES_PER_WG). Thread t takes a
 // contiguous run of sequences, so one wave scan plus the waves' totals give every prefix.
+template <bool MOD = false>
 __device__ void stage_batch(const DecodeArgs& a, BatchLds& s) {
   const int tid = threadIdx.x, nt = blockDim.x;
   const int lane = tid & (kWave - 1), wave = tid / kWave;
@@ -307,11 +336,12 @@ __device__ void stage_batch(const DecodeArgs& a, BatchLds& s) {
   const int b0 = tid * per, b1 = min(a.batch, b0 + per);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) {
-    const int fb = first_blk(a, b);
-    const int n = clamped_ctx(a, b);
+    const int fb = first_blk<MOD>(a, b);
+    const int n = clamped_ctx<MOD>(a, b);
     s.n[b] = n;
     s.fb[b] = fb;
-    s.pre[b] = a.pre_row ? a.pre_row[b] : -1;
+    if constexpr (MOD) s.pre[b] = key_span(a, b).lo - fb * a.bs;  // no cascade: the first key
+    else s.pre[b] = a.pre_row ? a.pre_row[b] : -1;
     mine += units_of(a, n);
   }
   int64_t incl = mine;
@@ -346,9 +376,11 @@ __device__ __forceinline__ int staged_owner(const DecodeArgs& a, const BatchLds&
 // ROWS: a.rows may be non-null. A form of its own: with the lookup at run time the plain one took 2
 // registers more (fp32 at head_dim 64, 4 heads: 173, a wave per SIMD less), and 64 sequences of
 // 100-919 tokens, 16 / 2 heads, hd 256, bf16 38.7 us against 37.0.
-template <int DT, int HD, int GPW, bool ROWS>
+// MOD (modified scores): with ROWS, and a.rows may be null.
+template <int DT, int HD, int GPW, bool ROWS, bool MOD = false>
 __global__ void __launch_bounds__(512)
 paged_decode_stream_kernel(const DecodeArgs a) {
+  static_assert(!MOD || ROWS, "modified scores take the row lookup");
   using Sh = DecodeShape<DT, HD>;
   constexpr int VEC = Sh::VEC, LPT = Sh::LPT, TPL = Sh::TPL, NLOAD = Sh::NLOAD;
   constexpr int TILE = Sh::TILE;
@@ -362,7 +394,7 @@ paged_decode_stream_kernel(const DecodeArgs a) {
   const int w = blockIdx.x;
 
   int64_t total, rs, re, ub;
-  int b = locate_range(a, w, &total, &rs, &re, &ub);
+  int b = locate_range<MOD>(a, w, &total, &rs, &re, &ub);
   if (rs >= re) return;
 
   const int row = lane / LPT;         // token sub-index inside a load
@@ -371,7 +403,7 @@ paged_decode_stream_kernel(const DecodeArgs a) {
   const S* vbase = reinterpret_cast<const S*>(a.v) + (int64_t)kvh * a.kv_sh + d0;
 
   for (int64_t u = rs; u < re && b < a.batch; ++b) {
-    const int n = clamped_ctx(a, b);
+    const int n = clamped_ctx<MOD>(a, b);
     const int64_t ue = ub + units_of(a, n);
     const int64_t seg_end = ue < re ? ue : re;
     const bool whole = (u == ub) && (seg_end == ue);
@@ -397,8 +429,17 @@ paged_decode_stream_kernel(const DecodeArgs a) {
 
     // Block ids of up to 64 consecutive blocks starting at cb, one per lane.
     int cb = 0, tbl = 0;
-    const int fb = first_blk(a, b);
+    const int fb = first_blk<MOD>(a, b);
     const int pre_b = a.pre_row ? a.pre_row[b] : -1;  // cascade: b's prefix row, or none
+    // MOD: the range's first key and the query's position, counted from column fb's first token.
+    int lo = 0, qpos = 0;
+    float slope[GPW];
+    if constexpr (MOD) {
+      lo = key_span(a, b).lo - fb * a.bs;
+      qpos = min(max(a.ctx[b], 0), a.max_blocks * a.bs) - 1 - fb * a.bs;
+#pragma unroll
+      for (int g = 0; g < GPW; ++g) slope[g] = a.mod.slopes ? a.mod.slopes[h0 + g] * kLog2e : 0.f;
+    }
     auto load_table = [&](int first_block) {
       cb = first_block;
       const int j = cb + lane;
@@ -413,7 +454,7 @@ paged_decode_stream_kernel(const DecodeArgs a) {
       const int bid = __shfl(tbl, blk - cb);
       const int off = p - blk * a.bs;
       const int64_t sl = (int64_t)bid * a.bs + off;
-      return (p < t1 && sl >= 0 && sl < a.num_slots) ? sl : (int64_t)-1;
+      return (p < t1 && (!MOD || p >= lo) && sl >= 0 && sl < a.num_slots) ? sl : (int64_t)-1;
     };
     // Issue the K/V loads of the tile at tb (first making sure the table window
     // covers it); bit i of the result: load i holds a live token for this lane.
@@ -470,6 +511,10 @@ paged_decode_stream_kernel(const DecodeArgs a) {
           float mx = -INFINITY;
 #pragma unroll
           for (int i = 0; i < NLOAD; ++i) {
+            if constexpr (MOD) {
+              if (a.mod.c2 != 0.f) sc[i][g] = capped<DT == PKV_F32>(a.mod, sc[i][g]);
+              if (a.mod.slopes) sc[i][g] = biased(sc[i][g], slope[g], qpos - (tb + i * TPL + row));
+            }
             sc[i][g] = ((okc >> i) & 1u) ? sc[i][g] : -INFINITY;
             mx = fmaxf(mx, sc[i][g]);
           }
@@ -666,7 +711,7 @@ constexpr int kSplitMaxColumns = 2048;  // table columns staged in LDS
 // The split pass's merge: every wave's state (lanes grp == 0, col < HD / 8 hold acc[g]
 // for head dims 8 col .. 8 col + 7; lh, mh are the same in every lane) goes to LDS, then
 // wave g < GPW merges query head h0 + g and stores it. All waves call it.
-template <int DT, int GPW, int HD>
+template <int DT, int GPW, int HD, bool MOD>
 __device__ __forceinline__ void split_merge(const DecodeArgs& a, int b, int h0,
                                             const float (&acc)[GPW][8], const float (&lh)[GPW],
                                             const float (&mh)[GPW]) {
@@ -710,6 +755,7 @@ __device__ __forceinline__ void split_merge(const DecodeArgs& a, int b, int h0,
   const int64_t srow = seq_row(a, b);
   if (srow < 0) return;
   const int64_t e = srow * a.out_sb + (int64_t)(h0 + g) * a.out_sh + DPL * lane;
+  if (MOD && a.lse && lane == 0) a.lse[(int64_t)b * a.nh + h0 + g] = lse_of(mmax, l);
 #pragma unroll
   for (int k = 0; k < DPL; ++k) {
     const float v = o[k] * inv;
@@ -721,7 +767,7 @@ __device__ __forceinline__ void split_merge(const DecodeArgs& a, int b, int h0,
 // The same for the wide form, whose states are O^T (head col's dims 16 d + 4 grp .. + 3 in
 // lane (col, grp)): kSplitWaves heads at a time through the V slots (free once every wave has
 // passed its last tile), head g0 + w merged by wave w. ng is the workgroup's.
-template <int DT, int HD>
+template <int DT, int HD, bool MOD>
 __device__ __forceinline__ void split_merge_wide(const DecodeArgs& a, int b, int h0, int ng,
                                                  const f32x4 (&ov)[HD / 16], float o_scale,
                                                  float l_own, float m_own, u32x4* vslots) {
@@ -763,6 +809,7 @@ __device__ __forceinline__ void split_merge_wide(const DecodeArgs& a, int b, int
         o[k] = __builtin_fmaf(wgt, part[(s * W + wave) * HD + DPL * lane + k], o[k]);
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;  // empty context: 0
+    if (MOD && a.lse && lane == 0) a.lse[(int64_t)b * a.nh + h0 + g] = lse_of(mmax, l);
     const int64_t e = srow * a.out_sb + (int64_t)(h0 + g) * a.out_sh + DPL * lane;
 #pragma unroll
     for (int k = 0; k < DPL; ++k) {
@@ -778,10 +825,11 @@ __device__ __forceinline__ void split_merge_wide(const DecodeArgs& a, int b, int
 // matrix cores (pv_mfma), else unused.
 // ROWS: a.rows may be non-null (always looked at in the split pass).
 template <int DT, int GPW, bool FAST, int HD, bool SPLIT, bool STAGED = false, bool WT = false,
-          bool ROWS = false>
+          bool ROWS = false, bool MOD = false>
 __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int bx, const int by,
                                                  u32x4* const vslots) {
   static_assert(!WT || STAGED, "the one-launch cascade's split takes the staged pass");
+  static_assert(!MOD || ((ROWS || SPLIT) && !WT), "modified scores take the row lookup, no cascade");
   // hd 128: a step is one 16-token tile, four 32-dim MFMA k-blocks, V rows over all 16
   // lane columns (8 dims each). hd 64: a step is two 16-token sub-tiles (the same 8 KB
   // per wave in flight as at hd 128), two k-blocks each, the V rows of sub-tile u on
@@ -847,19 +895,19 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
     total = rs = ub = 0;
     re = 1;
     b = bx;
-    split_n = clamped_ctx(a, b);
+    split_n = clamped_ctx<MOD>(a, b);
     for (int j = threadIdx.x; j < a.max_blocks; j += blockDim.x)
       split_table[j] = a.tables[(int64_t)b * a.table_stride + j];
     __syncthreads();
   } else if constexpr (STAGED) {  // every wave of the workgroup stages, then idle ones leave
-    stage_batch(a, batch_lds[0]);
+    stage_batch<MOD>(a, batch_lds[0]);
     total = batch_lds[0].ub[a.batch];
     rs = range_start<WT>(a, w, total);
     re = range_start<WT>(a, w + 1, total);
     b = rs < re ? staged_owner(a, batch_lds[0], rs) : a.batch;
     ub = rs < re ? batch_lds[0].ub[b] : 0;
   } else {
-    b = locate_range(a, w, &total, &rs, &re, &ub);
+    b = locate_range<MOD>(a, w, &total, &rs, &re, &ub);
   }
   if (STAGED && kvh >= a.nkv) return;
   if (rs >= re) return;
@@ -877,7 +925,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
   for (int64_t u = rs; u < re && b < a.batch; ++b) {
     int n;
     if constexpr (SPLIT) n = split_n;
-    else n = staged ? batch_lds[0].n[b] : clamped_ctx(a, b);
+    else n = staged ? batch_lds[0].n[b] : clamped_ctx<MOD>(a, b);
     int t0, t1, slot = 0;
     bool whole = true;
     if constexpr (SPLIT) {  // this wave's 16-token-aligned share of the context
@@ -920,14 +968,33 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
     }
 
     int cb = 0, tbl = 0;
-    const int fb = staged ? batch_lds[0].fb[b] : first_blk(a, b);
+    const int fb = staged ? batch_lds[0].fb[b] : first_blk<MOD>(a, b);
     // cascade: b's prefix row, or none
-    const int pre_b = staged ? batch_lds[0].pre[b] : (a.pre_row ? a.pre_row[b] : -1);
+    const int pre_b = MOD ? -1 : staged ? batch_lds[0].pre[b] : (a.pre_row ? a.pre_row[b] : -1);
+    // MOD: the range's first key and the query's position, counted from column fb's first token
+    // (lo is wave-uniform, as t0 and t1 are), and this lane's head's slope.
+    int lo = 0, qpos = 0;
+    float slope = 0.f;
+    if constexpr (MOD) {
+      lo = staged ? batch_lds[0].pre[b] : key_span(a, b).lo - fb * a.bs;
+      lo = __builtin_amdgcn_readfirstlane(lo);
+      qpos = min(max(a.ctx[b], 0), a.max_blocks * a.bs) - 1 - fb * a.bs;
+      if (a.mod.slopes && col < ng) slope = a.mod.slopes[h0 + col] * kLog2e;
+    }
+    // The score of the key at position p (from column fb) for this lane's head.
+    auto modified = [&](float s, int p) __attribute__((always_inline)) {
+      s *= a.scale_log2;
+      if constexpr (MOD) {
+        if (a.mod.c2 != 0.f) s = capped<false>(a.mod, s);
+        if (a.mod.slopes) s = biased(s, slope, qpos - p);
+      }
+      return s;
+    };
     auto load_table = [&](int first_block) {
       cb = first_block;
       const int j = cb + lane;
-      if constexpr (SPLIT)  // first_block is null on the split path: fb == 0
-        tbl = j < a.max_blocks ? split_table[j] : 0;
+      if constexpr (SPLIT)  // without MOD first_block is null on the split path: fb == 0
+        tbl = j < a.max_blocks - (MOD ? fb : 0) ? split_table[j + (MOD ? fb : 0)] : 0;
       else
         tbl = j < a.max_blocks - fb ? a.tables[b * a.table_stride + fb + j] : 0;
     };
@@ -948,10 +1015,12 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
         const int blk = block_of(tb);
         const int bid = __builtin_amdgcn_readlane(tbl, blk - cb);
         const int64_t slot0 = (int64_t)bid * a.bs + (tb - blk * a.bs);
-        const int live = (bid >= 0 && slot0 + TILE <= a.num_slots) ? min(TILE, t1 - tb) : 0;
+        int live = (bid >= 0 && slot0 + TILE <= a.num_slots) ? min(TILE, t1 - tb) : 0;
+        const int skip = MOD ? max(0, lo - tb) : 0;  // tokens before the range
+        if (MOD && skip >= live) live = 0;
         const S* kt = kbase + slot0 * a.kv_ss;
         const S* vt = vbase + slot0 * a.kv_ss;
-        if (live == TILE) {  // full tile: every lane loads, no predication
+        if (live == TILE && (!MOD || skip == 0)) {  // full tile: every lane loads, no predication
 #pragma unroll
           for (int m = 0; m < KB; ++m) kr[m] = load_kv16v(kt + k_off + 32 * m);
 #pragma unroll
@@ -965,15 +1034,17 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
         }
         // Last, partial tile of a piece: lanes past the end re-read the last live
         // token (finite data) and are masked out of the softmax (P = 0).
-        const int kt_tok = min(col, live - 1);
+        // Those before the range (MOD) read its first token.
+        const int kt_tok = MOD ? max(min(col, live - 1), skip) : min(col, live - 1);
 #pragma unroll
         for (int m = 0; m < KB; ++m)
           kr[m] = load_kv16v(kt + kt_tok * a.kv_ss + 8 * grp + 32 * m);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int tok = 4 * grp + r;
-          vr[r] = col < VC ? load_kv16v(vt + min(tok, live - 1) * a.kv_ss + 8 * col) : z;
-          ok |= (unsigned)(tok < live) << r;
+          const int vt_tok = MOD ? max(min(tok, live - 1), skip) : min(tok, live - 1);
+          vr[r] = col < VC ? load_kv16v(vt + vt_tok * a.kv_ss + 8 * col) : z;
+          ok |= (unsigned)(tok < live && (!MOD || tok >= skip)) << r;
         }
       } else {
         // K token tb + col; the V lanes fetch their tokens' slots from those lanes.
@@ -981,7 +1052,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
         const int blk = block_of(p);
         const int bid = __shfl(tbl, blk - cb);
         const int64_t sl = (int64_t)bid * a.bs + (p - blk * a.bs);
-        const bool kon = p < t1 && sl >= 0 && sl < a.num_slots;
+        const bool kon = p < t1 && (!MOD || p >= lo) && sl >= 0 && sl < a.num_slots;
         const int64_t kslot = kon ? sl : -1;
 #pragma unroll
         for (int m = 0; m < KB; ++m)
@@ -1021,7 +1092,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
       if constexpr (FAST) {
         // One load form for full and partial sub-tiles (token index clamped to the last
         // live one), so the only branches are on the wave-uniform live counts.
-        int live[2];
+        int live[2], skip[2];
         const S* vt[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -1030,15 +1101,19 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
           const int bid = __builtin_amdgcn_readlane(tbl, blk - cb);
           const int64_t slot0 = (int64_t)bid * a.bs + (tu - blk * a.bs);
           live[u] = (tu < t1 && bid >= 0 && slot0 + TILE <= a.num_slots) ? min(TILE, t1 - tu) : 0;
+          skip[u] = MOD ? max(0, lo - tu) : 0;  // tokens before the range
+          if (MOD && skip[u] >= live[u]) live[u] = 0;
           // a dead sub-tile's lanes read pool row 0 (in bounds when any tile is live) and
           // are masked out
           vt[u] = vbase + (live[u] ? slot0 : 0) * a.kv_ss;
           if (live[u] > 0) {
-            const S* kt = kbase + slot0 * a.kv_ss + min(col, live[u] - 1) * a.kv_ss + 8 * grp;
+            const int kt_tok = MOD ? max(min(col, live[u] - 1), skip[u]) : min(col, live[u] - 1);
+            const S* kt = kbase + slot0 * a.kv_ss + kt_tok * a.kv_ss + 8 * grp;
 #pragma unroll
             for (int m = 0; m < KB; ++m) kr[KB * u + m] = load_kv16v(kt + 32 * m);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) ok |= (unsigned)(4 * grp + r < live[u]) << (4 * u + r);
+            for (int r = 0; r < 4; ++r)
+              ok |= (unsigned)(4 * grp + r < live[u] && (!MOD || 4 * grp + r >= skip[u])) << (4 * u + r);
           } else {
 #pragma unroll
             for (int m = 0; m < KB; ++m) kr[KB * u + m] = z;
@@ -1047,8 +1122,13 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
         if (live[0] + live[1] > 0) {
           const S* vl = vlane0 ? vt[0] : vt[1];
           const int lv = max(vlane0 ? live[0] : live[1], 1);
+          // a dead sub-tile reads row 0 whatever its skip
+          const int sk = MOD ? min(vlane0 ? skip[0] : skip[1], lv - 1) : 0;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) vr[r] = load_kv16v(vl + min(4 * grp + r, lv - 1) * a.kv_ss + vd);
+          for (int r = 0; r < 4; ++r) {
+            const int vt_tok = MOD ? max(min(4 * grp + r, lv - 1), sk) : min(4 * grp + r, lv - 1);
+            vr[r] = load_kv16v(vl + vt_tok * a.kv_ss + vd);
+          }
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r) vr[r] = z;
@@ -1061,7 +1141,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
           const int blk = block_of(p);
           const int bid = __shfl(tbl, blk - cb);
           const int64_t sl = (int64_t)bid * a.bs + (p - blk * a.bs);
-          const bool kon = p < t1 && sl >= 0 && sl < a.num_slots;
+          const bool kon = p < t1 && (!MOD || p >= lo) && sl >= 0 && sl < a.num_slots;
           kslot[u] = kon ? sl : -1;
 #pragma unroll
           for (int m = 0; m < KB; ++m)
@@ -1129,7 +1209,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
       }
       return m_run == -INFINITY ? 0.f : m_run;
     };
-    auto tile = [&](const u32x4* kr, const u32x4* vr, unsigned ok) {
+    auto tile = [&](const u32x4* kr, const u32x4* vr, unsigned ok, [[maybe_unused]] int tb) {
       if constexpr (NS == 1) {
         // PVM: V row 4 grp + r goes to the wave's slot, chunk col at (col ^ swz(row)), swz(t)
         // = (t3, t0, t1, t2) as in the prefill's tiles, and comes back as V^T fragments:
@@ -1157,7 +1237,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
         float mx = -INFINITY;
   #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[r] = ((ok >> r) & 1u) ? s[r] * a.scale_log2 : -INFINITY;
+          p[r] = ((ok >> r) & 1u) ? modified(s[r], tb + 4 * grp + r) : -INFINITY;
           mx = fmaxf(mx, p[r]);
         }
         const float mref = raise_ref(rows_max(mx));
@@ -1249,7 +1329,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
           for (int m = 0; m < KB; ++m) s = MMA::mma(kr[KB * u + m], qb[m], s);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            p[u][r] = ((ok >> (4 * u + r)) & 1u) ? s[r] * a.scale_log2 : -INFINITY;
+            p[u][r] = ((ok >> (4 * u + r)) & 1u) ? modified(s[r], tb + TILE * u + 4 * grp + r) : -INFINITY;
             mx = fmaxf(mx, p[u][r]);
           }
         }
@@ -1317,13 +1397,13 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
         unsigned ok2;
         for (int tb = t0; tb < t1; tb += 3 * STEP) {
           ok2 = load_step(tb + 2 * STEP, k2, v2);
-          tile(k0, v0, ok0);
+          tile(k0, v0, ok0, tb);
           if (tb + STEP >= t1) break;
           ok0 = load_step(tb + 3 * STEP, k0, v0);
-          tile(k1, v1, ok1);
+          tile(k1, v1, ok1, tb + STEP);
           if (tb + 2 * STEP >= t1) break;
           ok1 = load_step(tb + 4 * STEP, k1, v1);
-          tile(k2, v2, ok2);
+          tile(k2, v2, ok2, tb + 2 * STEP);
         }
       } else {
         // Two tile buffers in ping-pong: the next tile is in flight while one is reduced.
@@ -1331,10 +1411,10 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
         unsigned oka = load_step(t0, ka, va);
         for (int tb = t0; tb < t1; tb += 2 * STEP) {
           const unsigned okb = load_step(tb + STEP, kb2, vb2);
-          tile(ka, va, oka);
+          tile(ka, va, oka, tb);
           if (tb + STEP >= t1) break;
           oka = load_step(tb + 2 * STEP, ka, va);
-          tile(kb2, vb2, okb);
+          tile(kb2, vb2, okb, tb + STEP);
         }
       }
     }
@@ -1356,7 +1436,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
       // grp .. + 3 of head h0 + col, and stores them as they are.
       constexpr float kOScale = DT == PKV_F16 && HD == 64 ? 1.f / 128.f : 1.f;  // P's fp16 scale undone
       if constexpr (SPLIT) {
-        split_merge_wide<DT, HD>(a, b, h0, ng, ov, kOScale, l_tot, m_run, vslots);
+        split_merge_wide<DT, HD, MOD>(a, b, h0, ng, ov, kOScale, l_tot, m_run, vslots);
         return;
       }
       if (col < ng) {
@@ -1401,7 +1481,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
     }
 
     if constexpr (SPLIT) {
-      split_merge<DT, GPW, HD>(a, b, h0, acc, lh, mh);
+      split_merge<DT, GPW, HD, MOD>(a, b, h0, acc, lh, mh);
       return;
     }
     if (grp == 0 && col < VC) {  // lane c writes head dims 8c .. 8c + 7
@@ -1437,12 +1517,13 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeArgs& a, const int 
 }
 
 // Dynamic LDS: kVSlotBytes per wave where P.V runs on the matrix cores (pv_mfma).
-template <int DT, int GPW, bool FAST, int HD, bool SPLIT, bool STAGED = false, bool ROWS = false>
+template <int DT, int GPW, bool FAST, int HD, bool SPLIT, bool STAGED = false, bool ROWS = false,
+          bool MOD = false>
 __global__ void __launch_bounds__(512)
 paged_decode_mfma_kernel(const DecodeArgs a) {
   extern __shared__ __align__(16) u32x4 decode_vslots[];
-  decode_mfma_body<DT, GPW, FAST, HD, SPLIT, STAGED, false, ROWS>(a, (int)blockIdx.x,
-                                                                 (int)blockIdx.y, decode_vslots);
+  decode_mfma_body<DT, GPW, FAST, HD, SPLIT, STAGED, false, ROWS, MOD>(a, (int)blockIdx.x,
+                                                                      (int)blockIdx.y, decode_vslots);
 }
 
 // ---------------------------------------------------------------------------------
@@ -1461,13 +1542,14 @@ paged_decode_mfma_kernel(const DecodeArgs a) {
 // ---------------------------------------------------------------------------------
 
 // Total units, and the unit range [ub, ue) of sequence b, in one pass over the lengths.
+template <bool MOD = false>
 __device__ void seq_units(const DecodeArgs& a, int b, int64_t* ub, int64_t* ue, int64_t* total) {
   const int lane = threadIdx.x & (kWave - 1);
   int64_t before = 0, all = 0;
   int mine = 0;
   for (int c0 = 0; c0 < a.batch; c0 += kWave) {
     const int bb = c0 + lane;
-    const int cnt = bb < a.batch ? units_of(a, clamped_ctx(a, bb)) : 0;
+    const int cnt = bb < a.batch ? units_of(a, clamped_ctx<MOD>(a, bb)) : 0;
     int lt = bb < b ? cnt : 0;
     int tot = cnt;
     if (bb == b) mine = cnt;
@@ -1489,7 +1571,7 @@ __device__ void seq_units(const DecodeArgs& a, int b, int64_t* ub, int64_t* ue, 
 // SP = 1: one wave per (sequence, query head). SP > 1 (batches with few such pairs): SP
 // waves per pair, each folding its share of the records, their states merged through
 // LDS -- 1 / SP of the dependent round trips for a sequence cut into many pieces.
-template <int DT, int HD, int SP, bool WT = false, bool ROWS = false>
+template <int DT, int HD, int SP, bool WT = false, bool ROWS = false, bool MOD = false>
 __global__ void __launch_bounds__(SP > 4 ? SP * kWave : 256)
 paged_decode_combine_kernel(const DecodeArgs a) {
   static_assert(SP == 1 || SP == 2 || SP == 4 || SP == 8 || SP == 16, "waves per (sequence, head)");
@@ -1534,7 +1616,7 @@ paged_decode_combine_kernel(const DecodeArgs a) {
   const int64_t w0 = plan.x;
   // Units fewer than workgroups leave some ranges empty: then find the live ones.
   int64_t ub = 0, ue = 0, total = 0;
-  if (!plan.w) seq_units(a, b, &ub, &ue, &total);
+  if (!plan.w) seq_units<MOD>(a, b, &ub, &ue, &total);
   const int64_t row0 = (w0 * 2 + plan.z) * a.nh + h;  // record 0: always live
 
   float out_acc[DPL], lsum = 0.f, mmax = -INFINITY;

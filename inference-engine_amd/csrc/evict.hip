@@ -1,0 +1,352 @@
+// evict.hip -- eviction from the paged pool by accumulated attention weight (include/paged_kv.h:
+// pkv_evict): every layer of a sequence keeps its last tokens and the heaviest of the others,
+// moved up in their order over the evicted ones' slots.
+
+#include "common.h"
+
+namespace {
+
+using namespace pkv;
+
+struct EvictArgs {
+  char* k;
+  char* v;
+  int64_t layer_bytes, row_bytes, num_slots;
+  float* w;  // layer l, row r, token p: w[l * w_layer + r * w_stride + p]
+  int64_t w_layer, w_stride, w_num;
+  const int64_t* w_rows;  // [batch] or null
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t max_blocks, bs, layers, batch, keep, recent;
+  const int32_t* ctx;
+  int32_t* new_ctx;
+  int2* head;   // [layers, batch]: first and one past the last token that moves
+  int2* moves;  // [layers, batch, keep]: (from, to) slots of kept token i, -1 outside the pool
+  int32_t keep_stride;
+};
+
+// ---------------------------------------------------------------------------------
+// Selection: one workgroup of 1,024 threads per (layer, sequence).
+//
+// Of the first n - recent tokens the k = keep - recent heaviest stay, ties by the lowest index.
+// Weights become unsigned keys in their order (NaN below all); the k-th largest key is built two
+// bits at a time from the top, each time by counting the keys at or above three candidates:
+// compares and scalar bit counts on keys in registers, and one barrier, instead of a histogram whose
+// LDS atomics would collide (weights share few exponents). Then rounds of 1,024 tokens in index
+// order give every kept token its place by prefix counts, move its weight there and leave its slots
+// for the move pass. R: keys per thread in registers while they are counted (R = 0: more tokens
+// than that, read from L2 in every counting round).
+// ---------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t weight_key(float x) {
+  if (x != x) return 0u;
+  const uint32_t u = __float_as_uint(x + 0.f);  // -0 is 0
+  return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / kWave;
+
+template <int R>
+__global__ void __launch_bounds__(kSelThreads)
+evict_select_kernel(const EvictArgs a) {
+  __shared__ int counts[2][kSelWaves][4];
+  __shared__ int first_gap;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int b = blockIdx.x % a.batch, layer = blockIdx.x / a.batch;
+  const int cap = a.max_blocks * a.bs;
+  const int n = min(max(a.ctx[b], 0), cap);
+  const int64_t wrow = a.w_rows ? a.w_rows[b] : b;
+  const bool skip = wrow < 0 || wrow >= a.w_num;
+  int2* head = a.head + (int64_t)layer * a.batch + b;
+  if (layer == 0 && tid == 0) a.new_ctx[b] = skip ? a.ctx[b] : min(n, a.keep);
+  if (skip || n <= a.keep) {  // uniform: nothing to evict
+    if (tid == 0) *head = make_int2(0, 0);
+    return;
+  }
+  float* w = a.w + layer * a.w_layer + wrow * a.w_stride;
+  const int old = n - a.recent, k = a.keep - a.recent;  // 0 <= k < old
+  const int rounds = (n + kSelThreads - 1) / kSelThreads;
+
+  constexpr int RR = R > 0 ? R : 1;
+  float x[RR];
+  uint32_t key[RR];
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int i = j * kSelThreads + tid;
+      x[j] = i < n ? w[i] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) key[j] = weight_key(x[j]);
+  }
+  if (tid == 0) first_gap = n;
+
+  // The largest key t with at least k keys >= t among the old tokens (k > 0).
+  uint32_t t = 0;
+  int above = 0;  // keys >= t + (the unit of the last two bits decided): in the end keys > t
+  if (k > 0) {
+    for (int bit = 30; bit >= 0; bit -= 2) {
+      const uint32_t c1 = t | (1u << bit), c2 = t | (2u << bit), c3 = t | (3u << bit);
+      int n1 = 0, n2 = 0, n3 = 0;
+      auto count = [&](int i, uint32_t kk) __attribute__((always_inline)) {
+        const bool in = i < old;
+        n1 += __popcll(__ballot(in && kk >= c1));
+        n2 += __popcll(__ballot(in && kk >= c2));
+        n3 += __popcll(__ballot(in && kk >= c3));
+      };
+      if constexpr (R > 0) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) count(j * kSelThreads + tid, key[j]);
+      } else {
+        for (int j = 0; j < rounds; ++j) {
+          const int i = j * kSelThreads + tid;
+          count(i, i < old ? weight_key(w[i]) : 0u);
+        }
+      }
+      int(*cnt)[4] = counts[(bit >> 1) & 1];  // two buffers: one barrier a round
+      if (lane == 0) {
+        cnt[wave][0] = n1;
+        cnt[wave][1] = n2;
+        cnt[wave][2] = n3;
+      }
+      __syncthreads();
+      int m1 = 0, m2 = 0, m3 = 0;
+#pragma unroll
+      for (int s = 0; s < kSelWaves; ++s) {
+        m1 += cnt[s][0];
+        m2 += cnt[s][1];
+        m3 += cnt[s][2];
+      }
+      // at(t) >= k holds; t grows to the largest candidate for which it still does
+      if (m3 >= k) t = c3;
+      else if (m2 >= k) t = c2, above = m3;
+      else if (m1 >= k) t = c1, above = m2;
+      else above = m1;
+      t = (uint32_t)__builtin_amdgcn_readfirstlane((int)t);
+    }
+  }
+  const int ties = k - above;  // tokens equal to t that stay, the first ones
+
+  __syncthreads();
+  const int32_t* trow = a.tables + (int64_t)b * a.table_stride;
+  auto slot_of = [&](int p) {
+    const int id = trow[p / a.bs];
+    const int64_t sl = (int64_t)id * a.bs + p % a.bs;
+    return id >= 0 && sl < a.num_slots ? (int)sl : -1;  // num_slots < 2^31 (launch)
+  };
+  int2* moves = a.moves + ((int64_t)layer * a.batch + b) * a.keep_stride;
+  int before = 0, eq_before = 0;  // tokens kept for sure, and tokens equal to t, in earlier rounds
+  auto emit = [&](int j, float xv, uint32_t kk) __attribute__((always_inline)) {
+    const int i = j * kSelThreads + tid;
+    const bool sure = (i < old && k > 0 && kk > t) || (i >= old && i < n);
+    const bool eq = i < old && k > 0 && kk == t;
+    const uint64_t bs = __ballot(sure), be = __ballot(eq);
+    int(*cnt)[4] = counts[j & 1];
+    if (lane == 0) {
+      cnt[wave][0] = __popcll(bs);
+      cnt[wave][1] = __popcll(be);
+    }
+    __syncthreads();  // the round's weights are in registers; the earlier rounds' moves may be overtaken
+    int sb = before, eb = eq_before, st = 0, et = 0;
+#pragma unroll
+    for (int s = 0; s < kSelWaves; ++s) {
+      const int cs = cnt[s][0], ce = cnt[s][1];
+      if (s < wave) sb += cs, eb += ce;
+      st += cs;
+      et += ce;
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    sb += __popcll(bs & below);
+    eb += __popcll(be & below);
+    const int pos = sb + min(eb, ties);
+    const bool kept = sure || (eq && eb < ties);
+    if (kept) {
+      w[pos] = xv;
+      moves[pos] = make_int2(slot_of(i), slot_of(pos));
+    } else if (i < n) {
+      atomicMin(&first_gap, i);
+    }
+    before += st;
+    eq_before += et;
+  };
+  if constexpr (R > 0 && R <= 4) {
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (j < rounds) emit(j, x[j], key[j]);
+  } else {  // read again: no round before wrote past its own tokens
+    for (int j = 0; j < rounds; ++j) {
+      const int i = j * kSelThreads + tid;
+      const float xv = i < n ? w[i] : 0.f;
+      emit(j, xv, weight_key(xv));
+    }
+  }
+  __syncthreads();
+  for (int i = a.keep + tid; i < n; i += kSelThreads) w[i] = 0.f;
+  if (tid == 0) *head = make_int2(first_gap, a.keep);
+}
+
+// ---------------------------------------------------------------------------------
+// Move: kept token i goes from its slot to token i's, for every i from the first gap on.
+//
+// A token moves down (from >= to), and moves go up in i, so in one wave that reads a batch of
+// tokens before it writes them, and takes the batches in order, nothing is overwritten unread: a
+// later batch's sources lie at or past every earlier batch's destinations. The bytes of a row are
+// independent, so a wave takes a slice of SLICE bytes of every row of one (layer, sequence, K or V)
+// and needs no other wave. The next batch's rows are on their way while this one's are written.
+// Bound by HBM, every row read and written once.
+// ---------------------------------------------------------------------------------
+
+template <int SLICE>
+__global__ void __launch_bounds__(256)
+evict_move_kernel(const EvictArgs a, int slices) {
+  constexpr int LPR = SLICE / 16;      // lanes per row
+  constexpr int RPL = kWave / LPR;     // rows per load
+  constexpr int U = 8;                 // loads per batch
+  constexpr int BATCH = RPL * U;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t job = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;  // slices innermost
+  const int64_t per = 2 * (int64_t)slices;
+  const int64_t seq = job / per;
+  if (seq >= (int64_t)a.layers * a.batch) return;
+  const int2 h = a.head[seq];
+  if (h.x >= h.y) return;
+  const int part = (int)(job % per);
+  const int slice = part % slices;
+  int64_t at = (int64_t)slice * SLICE + (lane % LPR) * 16;
+  const bool on = at < a.row_bytes;  // the last slice may be narrower
+  if (!on) at = 0;
+  char* pool = (part / slices ? a.v : a.k) + (seq / a.batch) * a.layer_bytes + at;
+  const int2* moves = a.moves + seq * a.keep_stride;
+  const int r = lane / LPR;
+
+  // Loads go out without conditions (a token past the end, a slot outside the pool and a lane past
+  // the row read slot 0), so that the wait for one batch does not wait for the next.
+  struct Moves {
+    int from[U], to[U];
+  };
+  auto load_moves = [&](int i0, Moves& m) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * RPL + r;
+      const int2 p = moves[min(i, h.y - 1)];
+      m.from[u] = p.x;
+      m.to[u] = i < h.y && p.x >= 0 ? p.y : -1;
+    }
+  };
+  auto load_rows = [&](const Moves& m, u32x4* d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      d[u] = *reinterpret_cast<const u32x4*>(pool + (int64_t)max(m.from[u], 0) * a.row_bytes);
+  };
+  Moves cur, next, after;
+  u32x4 x[U], nx[U];
+  load_moves(h.x, cur);
+  load_moves(h.x + BATCH, next);
+  load_rows(cur, x);
+  for (int i = h.x; i < h.y; i += BATCH) {
+    load_moves(i + 2 * BATCH, after);
+    load_rows(next, nx);
+    // Every row of this batch is in registers before any of it is overwritten: one statement that
+    // takes them all.
+    static_assert(U == 8, "the rows of a batch below");
+    __asm__ volatile("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]),
+                          "+v"(x[6]), "+v"(x[7]) : : "memory");
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (on && cur.to[u] >= 0) *reinterpret_cast<u32x4*>(pool + (int64_t)cur.to[u] * a.row_bytes) = x[u];
+    cur = next;
+    next = after;
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = nx[u];
+  }
+}
+
+struct EvictWs {
+  int64_t moves, total;
+};
+EvictWs evict_ws(int32_t layers, int32_t batch, int32_t keep) {
+  const int64_t pairs = (int64_t)layers * batch;
+  const int64_t moves = (pairs * 8 + 255) / 256 * 256;
+  return {moves, moves + pairs * keep * 8};
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t pkv_evict_workspace_bytes(int32_t layers, int32_t batch, int32_t max_blocks,
+                                  int32_t block_size, int32_t keep) {
+  if (layers < 0 || batch < 0 || max_blocks < 0 || block_size <= 0 || keep < 0 ||
+      (int64_t)max_blocks * block_size > (int64_t)1 << 30)
+    return PKV_E_SHAPE;
+  const int64_t cap = (int64_t)max_blocks * block_size;
+  return evict_ws(layers, batch, (int32_t)(keep < cap ? keep : cap)).total;
+}
+
+int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride_bytes, int32_t layers,
+              int64_t row_bytes, int64_t num_slots, float* weights, int64_t weight_stride_layer,
+              int64_t weight_stride_row, int64_t num_weight_rows, const int64_t* weight_rows,
+              const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+              int32_t block_size, const int32_t* context_lens, int32_t batch, int32_t keep,
+              int32_t recent, int32_t* new_lens, void* workspace, int64_t workspace_bytes,
+              void* stream) {
+  if (layers < 0 || layers > 65535 || batch < 0 || batch > (1 << 20) || block_size <= 0 ||
+      max_blocks < 0 || keep < 0 || recent < 0 || recent > keep || row_bytes <= 0 ||
+      num_slots < 0 || num_slots > 0x7FFFFFFF || num_weight_rows < 0)
+    return PKV_E_SHAPE;
+  if ((int64_t)max_blocks * block_size > (int64_t)1 << 30) return PKV_E_SHAPE;
+  if (!weight_rows && num_weight_rows < batch) return PKV_E_SHAPE;
+  if (layers == 0 || batch == 0) return 0;
+  if (!k_pool || !v_pool || !weights || !context_lens || !new_lens || !workspace ||
+      (max_blocks > 0 && !block_tables))
+    return PKV_E_NULL;
+  if (!aligned16(k_pool) || !aligned16(v_pool) || row_bytes % 16 || layer_stride_bytes % 16 ||
+      ((uintptr_t)workspace & 7u))
+    return PKV_E_ALIGN;
+  const int64_t cap = (int64_t)max_blocks * block_size;
+  const int32_t kept = (int32_t)(keep < cap ? keep : cap);  // the moves of one sequence
+  const EvictWs ws = evict_ws(layers, batch, kept);
+  if (workspace_bytes < ws.total) return PKV_E_WORKSPACE;
+  EvictArgs a;
+  a.k = (char*)k_pool;
+  a.v = (char*)v_pool;
+  a.layer_bytes = layer_stride_bytes;
+  a.row_bytes = row_bytes;
+  a.num_slots = num_slots;
+  a.w = weights;
+  a.w_layer = weight_stride_layer;
+  a.w_stride = weight_stride_row;
+  a.w_num = num_weight_rows;
+  a.w_rows = weight_rows;
+  a.tables = block_tables;
+  a.table_stride = table_stride;
+  a.max_blocks = max_blocks;
+  a.bs = block_size;
+  a.layers = layers;
+  a.batch = batch;
+  a.keep = keep;
+  a.recent = recent;
+  a.ctx = context_lens;
+  a.new_ctx = new_lens;
+  a.head = (int2*)workspace;
+  a.moves = (int2*)((char*)workspace + ws.moves);
+  a.keep_stride = kept;
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t seqs = (int64_t)layers * batch;
+  if (seqs > (1 << 22)) return PKV_E_SHAPE;  // 2^32 threads
+  const dim3 grid((unsigned)seqs), block(kSelThreads);
+  if (cap <= 4 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, st, a);
+  else if (cap <= 16 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<16>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || cap <= keep) return (int)e;
+  constexpr int SLICE = 64;
+  const int64_t slices = (row_bytes + SLICE - 1) / SLICE;
+  const int64_t wgs = (seqs * 2 * slices + 3) / 4;
+  if (slices > (1 << 20) || wgs >= ((int64_t)1 << 24)) return PKV_E_SHAPE;
+  hipLaunchKernelGGL(evict_move_kernel<SLICE>, dim3((unsigned)wgs), dim3(256), 0, st, a, (int)slices);
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

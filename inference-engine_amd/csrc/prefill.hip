@@ -6,6 +6,12 @@
 #include "cascade.h"
 #include "prefill_kernels.h"
 
+namespace pkv {
+// prefill_mod.hip: the 16-bit matrix-core kernel with modified scores.
+hipError_t launch_prefill_mod(const PrefillArgs& a, int kv_dtype, int head_dim, int64_t rows,
+                              hipStream_t st);
+}  // namespace pkv
+
 namespace {
 
 using namespace pkv;
@@ -48,7 +54,8 @@ template <int HD> struct F32Shape {
   static constexpr int BM = 64;         // query rows per workgroup
 };
 
-template <int DT, int HD>
+// MOD: modified scores (a.mod), as in prefill_body.
+template <int DT, int HD, bool MOD = false>
 __global__ void __launch_bounds__(512)
 paged_prefill_f32_kernel(const PrefillArgs a) {
   using SH = F32Shape<HD>;
@@ -80,18 +87,50 @@ paged_prefill_f32_kernel(const PrefillArgs a) {
   const int tok = min(rho, nrows - 1) / G, head = kvh * G + min(rho, nrows - 1) % G;
   int64_t qrow = q0 + tok;
   if (a.rows) qrow = token_row(a, qrow);
-  else if (a.q_rows) qrow = a.q_rows[q0 + tok];
+  else if (!MOD && a.q_rows) qrow = a.q_rows[q0 + tok];
   const bool row_ok = rho < nrows && qrow >= 0;  // no query: nothing read or written
   const int64_t orow = a.rows ? qrow : q0 + tok;
   const int last_row = min(nrows - 1, rho0 + BM - 1);
-  const int kend = a.causal ? min(n, base_pos + last_row / G + 1) : n;  // keys any row sees
-  const int limit = a.causal ? min(n - 1, base_pos + tok) : n - 1;      // last key of this row
+  int kend = a.causal ? min(n, base_pos + last_row / G + 1) : n;  // keys any row sees
+  int limit = a.causal ? min(n - 1, base_pos + tok) : n - 1;      // last key of this row
   // The last key of any row of this wave (its lane 15 holds the last row), -1 without rows: tiles
   // past it are only staged.
-  const int wlimit = rho0 + 16 * wave < nrows ? __builtin_amdgcn_readlane(limit, 15) : -1;
-  const int ntiles = kend > 0 ? (kend + TK - 1) / TK : 0;
+  int wlimit = rho0 + 16 * wave < nrows ? __builtin_amdgcn_readlane(limit, 15) : -1;
+  [[maybe_unused]] int first = 0, wfirst = 0;  // MOD: the first keys of this row and of the wave's
+  int kbeg = 0;
+  [[maybe_unused]] float slope = 0.f;
+  if constexpr (MOD) {
+    if (a.mod.slopes) slope = a.mod.slopes[head] * kLog2e;
+    if (a.mod.ranges) {
+      int beg = 0x7FFFFFFF, end = 0;
+      limit = -1;  // no query, or no key: nothing
+      if (row_ok) {
+        const int32_t* r = a.mod.ranges + qrow * a.mod.range_stride;
+        const int lo = max(r[0], 0), hi = min(r[1], n);
+        if (lo < hi) {
+          beg = first = lo;
+          end = hi;
+          limit = hi - 1;
+        }
+      }
+      const KeyBounds kb = key_bounds(beg, end, 0, 0, tid / kWave);
+      kbeg = min(kb.beg, kb.end);
+      kend = kb.end;
+      wlimit = limit;
+      wfirst = beg;
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) {
+        wlimit = max(wlimit, __shfl_xor(wlimit, off));
+        wfirst = min(wfirst, __shfl_xor(wfirst, off));
+      }
+      wlimit = __builtin_amdgcn_readfirstlane(wlimit);
+      wfirst = __builtin_amdgcn_readfirstlane(wfirst);
+    }
+  }
+  const int jbeg = MOD ? kbeg / TK : 0;  // first tile
+  const int ntiles = kend > 0 ? (kend + TK - 1) / TK - jbeg : 0;
   const int ns = (ntiles + 1) / 2;
-  const int tbeg = half ? ns : 0, nt = half ? ntiles - ns : ns;
+  const int tbeg = jbeg + (half ? ns : 0), nt = half ? ntiles - ns : ns;
 
   // Staging: chunk e = htid + 256 i of a tile is 16 bytes of row e / CPR.
   const int32_t* trow = a.tables + (int64_t)c * a.table_stride;
@@ -169,6 +208,7 @@ paged_prefill_f32_kernel(const PrefillArgs a) {
     load_kv(m + 1);
     load_ids(m + 2);
     if ((tbeg + m) * TK > wlimit) continue;  // wave-uniform
+    if (MOD && (tbeg + m + 1) * TK <= wfirst) continue;
     f32x4 sc[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) sc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -192,7 +232,11 @@ paged_prefill_f32_kernel(const PrefillArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int kpos = (tbeg + m) * TK + 16 * b + 4 * grp + r;
-        sc[b][r] = on[r] && kpos <= limit ? sc[b][r] : -INFINITY;
+        if constexpr (MOD) {
+          if (a.mod.c2 != 0.f) sc[b][r] = capped<true>(a.mod, sc[b][r]);
+          if (a.mod.slopes) sc[b][r] = biased(sc[b][r], slope, base_pos + tok - kpos);
+        }
+        sc[b][r] = on[r] && kpos <= limit && (!MOD || kpos >= first) ? sc[b][r] : -INFINITY;
         mx = fmaxf(mx, sc[b][r]);
       }
     }
@@ -263,6 +307,16 @@ paged_prefill_f32_kernel(const PrefillArgs a) {
   // whole wave, 64 keys at a time. Rare (V is finite in practice), so it is only kept small.
   uint64_t redo = __ballot(nan && row_ok);
   redo = (redo | redo >> 16 | redo >> 32 | redo >> 48) & 0xFFFF;
+  if constexpr (MOD) {
+    for (; redo; redo &= redo - 1) {
+      const int lr = __builtin_ctzll(redo);
+      const int r = rho0 + 16 * wave + lr;
+      redo_row<DT, HD>(a, it, r / G, r % G, __builtin_amdgcn_readlane((int)qrow, lr),
+                       __builtin_amdgcn_readlane(first, lr), __builtin_amdgcn_readlane(limit, lr),
+                       jbeg * TK, min(n, (jbeg + ntiles) * TK));
+    }
+    return;
+  }
   const int kused = min(kend, (wlimit / TK + 1) * TK);
   const S* kb = reinterpret_cast<const S*>(a.k) + (int64_t)kvh * a.kv_sh;
   const S* vb = reinterpret_cast<const S*>(a.v) + (int64_t)kvh * a.kv_sh;
@@ -388,7 +442,8 @@ hipError_t launch_v16(const PrefillArgs& a, int hd, hipStream_t st) {
 // The fp32 kernel: one workgroup per item (chunk, 64-row block, KV head). On two grid dimensions:
 // a bound on the chunks' lengths that few of them reach makes many empty items, and HIP launches
 // fewer than 2^32 threads along x.
-template <int DT, int HD> hipError_t launch_f32_hd(PrefillArgs a, int64_t rows, hipStream_t st) {
+template <int DT, int HD, bool MOD = false>
+hipError_t launch_f32_hd(PrefillArgs a, int64_t rows, hipStream_t st) {
   a.row_blocks = (int)((rows + F32Shape<HD>::BM - 1) / F32Shape<HD>::BM);
   const int64_t items = (int64_t)a.row_blocks * a.nkv * a.n_chunks;
   if (items > 0x7FFFFFFF) return hipErrorInvalidValue;
@@ -398,17 +453,17 @@ template <int DT, int HD> hipError_t launch_f32_hd(PrefillArgs a, int64_t rows, 
   // tokens, 32 / 8 heads, 352 items: 40.8 us against 46.2; 12 chunks of 3-599, 960: 452.6 against
   // 535 with one).
   const unsigned lds = HD == 64 && items < 512 ? 16384 : 0;
-  hipLaunchKernelGGL((paged_prefill_f32_kernel<DT, HD>),
+  hipLaunchKernelGGL((paged_prefill_f32_kernel<DT, HD, MOD>),
                      dim3((unsigned)gx, (unsigned)((items + gx - 1) / gx)), dim3(512), lds, st, a);
   return hipGetLastError();
 }
-hipError_t launch_f32(const PrefillArgs& a, int hd, int64_t rows, hipStream_t st) {
+template <bool MOD> hipError_t launch_f32(const PrefillArgs& a, int hd, int64_t rows, hipStream_t st) {
   switch (hd) {
-    case 16: return launch_f32_hd<PKV_F32, 16>(a, rows, st);
-    case 32: return launch_f32_hd<PKV_F32, 32>(a, rows, st);
-    case 64: return launch_f32_hd<PKV_F32, 64>(a, rows, st);
-    case 128: return launch_f32_hd<PKV_F32, 128>(a, rows, st);
-    default: return launch_f32_hd<PKV_F32, 256>(a, rows, st);
+    case 16: return launch_f32_hd<PKV_F32, 16, MOD>(a, rows, st);
+    case 32: return launch_f32_hd<PKV_F32, 32, MOD>(a, rows, st);
+    case 64: return launch_f32_hd<PKV_F32, 64, MOD>(a, rows, st);
+    case 128: return launch_f32_hd<PKV_F32, 128, MOD>(a, rows, st);
+    default: return launch_f32_hd<PKV_F32, 256, MOD>(a, rows, st);
   }
 }
 
@@ -482,6 +537,7 @@ int prefill_args(PrefillArgs* out_args, int64_t* rows_out, void* out, int out_dt
   a.v16_kstride = 0;
   a.rows = nullptr;
   a.rows_len = a.num_rows = 0;
+  a.mod = {0.f, 0.f, nullptr, nullptr, 0};
   return 0;
 }
 
@@ -492,7 +548,7 @@ namespace {
 // Launches for checked arguments: the 16-bit matrix-core kernel takes 16-bit K/V at head_dim
 // 32..256 (a bf16 call with a.v16 set converts the chunks' V first), the fp32 kernel the rest.
 int run_prefill(const PrefillArgs& a, int64_t rows, int kv_dtype, int head_dim, hipStream_t st) {
-  if (kv_dtype == PKV_F32) return (int)launch_f32(a, head_dim, rows, st);
+  if (kv_dtype == PKV_F32) return (int)launch_f32<false>(a, head_dim, rows, st);
   if (head_dim == 16)
     return (int)(kv_dtype == PKV_BF16 ? launch_f32_hd<PKV_BF16, 16>(a, rows, st)
                                       : launch_f32_hd<PKV_F16, 16>(a, rows, st));
@@ -505,6 +561,19 @@ int run_prefill(const PrefillArgs& a, int64_t rows, int kv_dtype, int head_dim, 
   }
   return (int)(a.rows ? launch_prefill<PKV_BF16, true>(a, head_dim, rows, st)
                       : launch_prefill<PKV_BF16, false>(a, head_dim, rows, st));
+}
+
+// The same with modified scores (a.mod).
+int run_prefill_mod(const PrefillArgs& a, int64_t rows, int kv_dtype, int head_dim, hipStream_t st) {
+  if (kv_dtype == PKV_F32) return (int)launch_f32<true>(a, head_dim, rows, st);
+  if (head_dim == 16)
+    return (int)(kv_dtype == PKV_BF16 ? launch_f32_hd<PKV_BF16, 16, true>(a, rows, st)
+                                      : launch_f32_hd<PKV_F16, 16, true>(a, rows, st));
+  if (a.v16) {
+    const hipError_t e = launch_v16(a, head_dim, st);
+    if (e != hipSuccess) return (int)e;
+  }
+  return (int)launch_prefill_mod(a, kv_dtype, head_dim, rows, st);
 }
 
 // Whether a call of these shapes can use the fp16 V copy: bf16 at head_dim 32..256,
@@ -528,6 +597,49 @@ V16Layout v16_layout(int32_t head_dim, int32_t num_kv_heads, int32_t n_chunks,
   l.k_bytes = ((int64_t)n_chunks * num_kv_heads * l.kstride + 255) / 256 * 256;
   l.total = l.k_bytes + (int64_t)n_chunks * pad * num_kv_heads * head_dim * 2;
   return l;
+}
+
+// pkv_paged_prefill_rows, with modified scores and the normalisers' destination (mod, lse null:
+// without).
+int prefill_rows(void* out, int out_dtype, int64_t out_stride_tok, int64_t out_stride_h,
+                 const void* q, int64_t q_stride_tok, int64_t q_stride_h, const void* k_cache,
+                 const void* v_cache, int kv_dtype, int64_t kv_stride_slot, int64_t kv_stride_head,
+                 int64_t num_slots, const int32_t* block_tables, int64_t table_stride,
+                 int32_t max_blocks, const int32_t* context_lens, const int32_t* cu_seqlens_q,
+                 int32_t n_chunks, int32_t max_query_len, int32_t num_heads, int32_t num_kv_heads,
+                 int32_t head_dim, int32_t block_size, float scale, void* workspace,
+                 int64_t workspace_bytes, const int64_t* rows, int64_t rows_len, int64_t num_rows,
+                 const ScoreMod* mod, float* lse, void* stream) {
+  if (rows_len < 0 || num_rows < 0 || num_rows > 0x7FFFFFFF) return PKV_E_SHAPE;
+  PrefillArgs a;
+  int64_t qrows = 0;  // query rows of the longest chunk for one KV head
+  const int bad = prefill_args(&a, &qrows, out, out_dtype, out_stride_tok, out_stride_h, q,
+                               q_stride_tok, q_stride_h, k_cache, v_cache, kv_dtype,
+                               kv_stride_slot, kv_stride_head, num_slots, block_tables,
+                               table_stride, max_blocks, context_lens, cu_seqlens_q, n_chunks,
+                               max_query_len, num_heads, num_kv_heads, head_dim, block_size,
+                               scale, 1, nullptr, lse);
+  if (bad) return bad == 1 ? 0 : bad;
+  if (rows) {
+    a.rows = rows;
+    a.rows_len = rows_len;
+    a.num_rows = num_rows;
+  }
+  if (workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return PKV_E_WORKSPACE;
+  if (workspace && !aligned16(workspace)) return PKV_E_ALIGN;
+  if (workspace && v16_shapes(kv_dtype, head_dim, max_blocks, block_size, num_slots)) {
+    const V16Layout l = v16_layout(head_dim, num_kv_heads, n_chunks, max_blocks, block_size);
+    if (workspace_bytes >= l.total) {
+      a.v16_k = static_cast<const uint8_t*>(workspace);
+      a.v16_kstride = (int32_t)l.kstride;
+      a.v16 = static_cast<const char*>(workspace) + l.k_bytes;
+    }
+  }
+  if (mod) {
+    a.mod = *mod;
+    return run_prefill_mod(a, qrows, kv_dtype, head_dim, (hipStream_t)stream);
+  }
+  return run_prefill(a, qrows, kv_dtype, head_dim, (hipStream_t)stream);
 }
 
 }  // namespace
@@ -611,32 +723,32 @@ int pkv_paged_prefill_rows(void* out, int out_dtype, int64_t out_stride_tok, int
                            float scale, void* workspace, int64_t workspace_bytes,
                            const int64_t* rows, int64_t rows_len, int64_t num_rows,
                            void* stream) {
-  if (rows_len < 0 || num_rows < 0 || num_rows > 0x7FFFFFFF) return PKV_E_SHAPE;
-  PrefillArgs a;
-  int64_t qrows = 0;  // query rows of the longest chunk for one KV head
-  const int bad = prefill_args(&a, &qrows, out, out_dtype, out_stride_tok, out_stride_h, q,
-                               q_stride_tok, q_stride_h, k_cache, v_cache, kv_dtype,
-                               kv_stride_slot, kv_stride_head, num_slots, block_tables,
-                               table_stride, max_blocks, context_lens, cu_seqlens_q, n_chunks,
-                               max_query_len, num_heads, num_kv_heads, head_dim, block_size,
-                               scale, 1, nullptr, nullptr);
-  if (bad) return bad == 1 ? 0 : bad;
-  if (rows) {
-    a.rows = rows;
-    a.rows_len = rows_len;
-    a.num_rows = num_rows;
-  }
-  if (workspace_bytes < 0 || (workspace_bytes > 0 && !workspace)) return PKV_E_WORKSPACE;
-  if (workspace && !aligned16(workspace)) return PKV_E_ALIGN;
-  if (workspace && v16_shapes(kv_dtype, head_dim, max_blocks, block_size, num_slots)) {
-    const V16Layout l = v16_layout(head_dim, num_kv_heads, n_chunks, max_blocks, block_size);
-    if (workspace_bytes >= l.total) {
-      a.v16_k = static_cast<const uint8_t*>(workspace);
-      a.v16_kstride = (int32_t)l.kstride;
-      a.v16 = static_cast<const char*>(workspace) + l.k_bytes;
-    }
-  }
-  return run_prefill(a, qrows, kv_dtype, head_dim, (hipStream_t)stream);
+  return prefill_rows(out, out_dtype, out_stride_tok, out_stride_h, q, q_stride_tok, q_stride_h,
+                      k_cache, v_cache, kv_dtype, kv_stride_slot, kv_stride_head, num_slots,
+                      block_tables, table_stride, max_blocks, context_lens, cu_seqlens_q, n_chunks,
+                      max_query_len, num_heads, num_kv_heads, head_dim, block_size, scale, workspace,
+                      workspace_bytes, rows, rows_len, num_rows, nullptr, nullptr, stream);
+}
+
+int pkv_paged_prefill_mod(void* out, int out_dtype, int64_t out_stride_tok, int64_t out_stride_h,
+                          const void* q, int64_t q_stride_tok, int64_t q_stride_h,
+                          const void* k_cache, const void* v_cache, int kv_dtype,
+                          int64_t kv_stride_slot, int64_t kv_stride_head, int64_t num_slots,
+                          const int32_t* block_tables, int64_t table_stride, int32_t max_blocks,
+                          const int32_t* context_lens, const int32_t* cu_seqlens_q, int32_t n_chunks,
+                          int32_t max_query_len, int32_t num_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t block_size, float scale, void* workspace,
+                          int64_t workspace_bytes, const int64_t* rows, int64_t rows_len,
+                          int64_t num_rows, float softcap, const float* alibi_slopes,
+                          const int32_t* key_ranges, int64_t range_stride, float* lse, void* stream) {
+  ScoreMod mod;
+  const int bad = score_mod(&mod, softcap, alibi_slopes, key_ranges, range_stride);
+  if (bad) return bad;
+  return prefill_rows(out, out_dtype, out_stride_tok, out_stride_h, q, q_stride_tok, q_stride_h,
+                      k_cache, v_cache, kv_dtype, kv_stride_slot, kv_stride_head, num_slots,
+                      block_tables, table_stride, max_blocks, context_lens, cu_seqlens_q, n_chunks,
+                      max_query_len, num_heads, num_kv_heads, head_dim, block_size, scale, workspace,
+                      workspace_bytes, rows, rows_len, num_rows, &mod, lse, stream);
 }
 
 }  // extern "C"

@@ -4,7 +4,7 @@
 
 #pragma once
 
-#include "common.h"
+#include "score_mod.h"
 
 namespace pkv {
 
@@ -45,6 +45,7 @@ struct PrefillArgs {
   // negative values count from the end, a row outside is skipped. Not with q_rows.
   const int64_t* rows;
   int64_t rows_len, num_rows;
+  ScoreMod mod;  // read by the kernels instantiated with MOD
 };
 
 // Query token t's row of q and out through `rows` (non-null), or -1.
@@ -350,6 +351,120 @@ struct PrefillItem {
   int c, q0, q1, n, kvh, rbi;
 };
 
+// MOD: over a workgroup's query rows with keys [first, last + 1), the smallest first and largest
+// end (the tiles to visit), and the largest first and smallest end (0 where a row has no keys):
+// tiles between these need no mask. beg, end, lo_m, hi_m: this lane's.
+struct KeyBounds {
+  int beg, end, lo_max, hi_min;
+};
+__device__ __forceinline__ KeyBounds key_bounds(int beg, int end, int lo_m, int hi_m, int wave) {
+  __shared__ int bounds[8][4];
+#pragma unroll
+  for (int off = 1; off < 16; off <<= 1) {  // the four rows of lanes hold the same query rows
+    beg = min(beg, __shfl_xor(beg, off));
+    end = max(end, __shfl_xor(end, off));
+    lo_m = max(lo_m, __shfl_xor(lo_m, off));
+    hi_m = min(hi_m, __shfl_xor(hi_m, off));
+  }
+  if ((threadIdx.x & (kWave - 1)) == 0) {
+    bounds[wave][0] = beg;
+    bounds[wave][1] = end;
+    bounds[wave][2] = lo_m;
+    bounds[wave][3] = hi_m;
+  }
+  __syncthreads();
+  KeyBounds k = {bounds[0][0], bounds[0][1], bounds[0][2], bounds[0][3]};
+#pragma unroll
+  for (int w = 1; w < 8; ++w) {
+    k.beg = min(k.beg, bounds[w][0]);
+    k.end = max(k.end, bounds[w][1]);
+    k.lo_max = max(k.lo_max, bounds[w][2]);
+    k.hi_min = min(k.hi_min, bounds[w][3]);
+  }
+  k.beg = __builtin_amdgcn_readfirstlane(k.beg);
+  k.end = __builtin_amdgcn_readfirstlane(k.end);
+  k.lo_max = __builtin_amdgcn_readfirstlane(k.lo_max);
+  k.hi_min = __builtin_amdgcn_readfirstlane(k.hi_min);
+  return k;
+}
+
+// A query row again, by one wave: token tok of the chunk, head j of KV head it.kvh's group, which
+// sees keys first .. last and whose tiles covered [beg, end). Keys that it does not see enter its
+// tiles' P.V with P = 0, and 0 x inf is NaN: where a V among them is infinite or NaN the row is
+// computed without them, 64 keys at a time, and stored at row `row` of out. Rare (V is finite in
+// practice), so it is only kept small. Every argument is wave-uniform.
+template <int DT, int HD>
+__device__ __forceinline__ void redo_row(const PrefillArgs& a, const PrefillItem& it, int tok, int j,
+                                      int64_t row, int first, int last, int beg, int end) {
+  using S = typename Elt<DT>::S;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int head = it.kvh * a.groups + j;
+  const int qpos = it.n - (it.q1 - it.q0) + tok;
+  const float slope = a.mod.slopes ? a.mod.slopes[head] * kLog2e : 0.f;
+  const int32_t* trow = a.tables + (int64_t)it.c * a.table_stride;
+  const S* qp = reinterpret_cast<const S*>(a.q) + row * a.q_st + (int64_t)head * a.q_sh;
+  const S* kb = reinterpret_cast<const S*>(a.k) + (int64_t)it.kvh * a.kv_sh;
+  const S* vb = reinterpret_cast<const S*>(a.v) + (int64_t)it.kvh * a.kv_sh;
+  auto slot_of = [&](int p) -> int64_t {  // key p's slot, -1 outside the pool
+    const int blk = a.bs_shift >= 0 ? p >> a.bs_shift : p / a.bs, id = trow[blk];
+    const int64_t sl = (int64_t)id * a.bs + (p - blk * a.bs);
+    return id >= 0 && sl < a.num_slots ? sl : -1;
+  };
+  bool bad = false;
+#pragma unroll 1
+  for (int p = beg + lane; p < end; p += kWave) {
+    if (p >= first && p <= last) continue;
+    int64_t sl = slot_of(p);
+    if (sl < 0) sl = 0;  // what the tiles read for it
+#pragma unroll 1
+    for (int e = 0; e < HD; ++e) bad = bad || !(fabsf(Elt<DT>::to_f32(vb[sl * a.kv_ss + e])) < INFINITY);
+  }
+  if (!__ballot(bad)) return;
+  auto score = [&](int p) {
+    const int64_t sl = p <= last ? slot_of(p) : -1;
+    if (sl < 0) return -INFINITY;
+    float d = 0.f;
+#pragma unroll 1
+    for (int e = 0; e < HD; ++e)
+      d = __builtin_fmaf(Elt<DT>::to_f32(qp[e]), Elt<DT>::to_f32(kb[sl * a.kv_ss + e]), d);
+    d *= a.scale_log2;
+    if (a.mod.c2 != 0.f) d = capped<DT == PKV_F32>(a.mod, d);
+    return a.mod.slopes ? biased(d, slope, qpos - p) : d;
+  };
+  constexpr int DPL = (HD + kWave - 1) / kWave;
+  float mr = -INFINITY, lr = 0.f, acc[DPL] = {};
+#pragma unroll 1
+  for (int p = first; p <= last; p += kWave) mr = fmaxf(mr, score(p + lane));
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) mr = fmaxf(mr, __shfl_xor(mr, off));
+#pragma unroll 1
+  for (int p = first; p <= last; p += kWave) {
+    const int64_t sl = p + lane <= last ? slot_of(p + lane) : -1;
+    const float pr = __builtin_amdgcn_exp2f(score(p + lane) - (mr == -INFINITY ? 0.f : mr));
+    lr += pr;
+#pragma unroll 1
+    for (int t = 0; t < kWave && p + t <= last; ++t) {
+      const int64_t st = __shfl(sl, t);
+      const float pt = __shfl(pr, t);
+#pragma unroll
+      for (int k = 0; k < DPL; ++k)
+        if (st >= 0 && lane + kWave * k < HD)
+          acc[k] = __builtin_fmaf(pt, Elt<DT>::to_f32(vb[st * a.kv_ss + lane + kWave * k]), acc[k]);
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) lr += __shfl_xor(lr, off);
+  const float inv = lr > 0.f ? 1.f / lr : 0.f;
+  const int64_t e0 = row * a.out_st + (int64_t)head * a.out_sh;
+#pragma unroll
+  for (int k = 0; k < DPL; ++k) {
+    const int d = lane + kWave * k;
+    if (d >= HD) break;
+    if (a.out_f32) reinterpret_cast<float*>(a.out)[e0 + d] = acc[k] * inv;
+    else reinterpret_cast<S*>(a.out)[e0 + d] = Elt<DT>::from_f32(acc[k] * inv);
+  }
+}
+
 // The K/V rings of an item: ring[half][0 = K, 1 = V][stage] holds each key half's K and V
 // tiles, two stages each; idring the block-table windows, per half and wave, in a ring
 // of three (one per tile in flight).
@@ -363,7 +478,9 @@ template <int HD> struct PrefillLds {
 // runs several items on one workgroup puts a barrier between them (the merge reuses the
 // rings).
 // ROWS: q and out rows through a.rows (else a.rows is null).
-template <int DT, int HD, bool POW2, bool V16, bool ROWS>
+// MOD: modified scores (a.mod), with ROWS, and a.rows may be null. Every query row then has its
+// own first and last key; the item's tiles run from the smallest to the largest of them.
+template <int DT, int HD, bool POW2, bool V16, bool ROWS, bool MOD = false>
 __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const PrefillItem& it,
                                              PrefillLds<HD>& lds) {
   using SH = PrefillShape<HD>;
@@ -371,6 +488,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   constexpr int NSG = SH::NSG, KS = SH::KS, DTL = SH::DTL, NLD = SH::NLD, TILE = SH::TILE;
   static_assert(HD % 32 == 0 && HD <= 256, "head_dim must be 32..256, a multiple of 32");
   static_assert(!V16 || DT == PKV_BF16, "the fp16 V copy serves bf16 caches");
+  static_assert(!MOD || ROWS, "modified scores take the row lookup");
   using MMA = Mfma16x16x32Bits<DT>;                   // Q.K^T
   using PM = Mfma16x16x32Bits<V16 ? PKV_F16 : DT>;    // P.V and the row sums
   using S = typename Elt<DT>::S;
@@ -405,7 +523,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
     row_tok[t] = rr / G;
     int64_t qrow = q0 + row_tok[t];
     if constexpr (ROWS) {
-      const int64_t r = token_row(a, qrow);
+      const int64_t r = MOD && !a.rows ? qrow : token_row(a, qrow);
       row_ok[t] = row_ok[t] && r >= 0;
       qrow = r >= 0 ? r : 0;
       row_out[t] = (int)qrow;
@@ -439,10 +557,47 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   // Keys any row of this workgroup attends to: [0, kend), in ntiles tiles; half 0 takes
   // tiles 0 .. ns - 1, half 1 the other ntiles - ns.
   const int last_row = min(nrows - 1, rho0 + BM - 1);
-  const int kend = a.causal ? min(n, base_pos + last_row / G + 1) : n;
-  const int ntiles = kend > 0 ? (kend + KT - 1) / KT : 0;
+  int kend = a.causal ? min(n, base_pos + last_row / G + 1) : n;
+  // MOD: rows' first and last keys, the tiles between the item's, and which tiles need no mask.
+  [[maybe_unused]] int mfirst[RT], mlast[RT];
+  int kbeg = 0;
+  [[maybe_unused]] int lo_max = 0, hi_min = 0;
+  if constexpr (MOD) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      mfirst[t] = 0;
+      mlast[t] = a.causal ? min(n - 1, base_pos + row_tok[t]) : n - 1;
+    }
+    hi_min = (a.causal ? min(n - 1, base_pos + rho0 / G) : n - 1) + 1;
+    if (a.mod.ranges) {
+      int beg = 0x7FFFFFFF, end = 0, lo_m = 0, hi_m = 0x7FFFFFFF;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        mlast[t] = -1;  // no query, or no key: nothing
+        if (row_ok[t]) {
+          const int32_t* r = a.mod.ranges + (int64_t)row_out[t] * a.mod.range_stride;
+          const int lo = max(r[0], 0), hi = min(r[1], n);
+          hi_m = min(hi_m, lo < hi ? hi : 0);
+          if (lo < hi) {
+            mfirst[t] = lo;
+            mlast[t] = hi - 1;
+            beg = min(beg, lo);
+            end = max(end, hi);
+            lo_m = max(lo_m, lo);
+          }
+        }
+      }
+      const KeyBounds kb = key_bounds(beg, end, lo_m, hi_m, tid / kWave);
+      kbeg = min(kb.beg, kb.end);
+      kend = kb.end;
+      lo_max = kb.lo_max;
+      hi_min = kb.hi_min;
+    }
+  }
+  const int jbeg = MOD ? kbeg / KT : 0;  // first tile
+  const int ntiles = kend > 0 ? (kend + KT - 1) / KT - jbeg : 0;
   const int ns = (ntiles + 1) / 2;
-  const int tbeg = half ? ns : 0;
+  const int tbeg = jbeg + (half ? ns : 0);
   const int nt = half ? ntiles - ns : ns;
 
   // Tile j's K (or V) rows go from the pool straight into LDS. Instruction r of wave w
@@ -661,7 +816,21 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   const int j_mask = min(ntiles, max(0, (limit_min + 1) / KT));
   int limit[RT];  // last key each of this lane's rows sees
 #pragma unroll
-  for (int t = 0; t < RT; ++t) limit[t] = a.causal ? min(n - 1, base_pos + row_tok[t]) : n - 1;
+  for (int t = 0; t < RT; ++t)
+    limit[t] = MOD ? mlast[t] : a.causal ? min(n - 1, base_pos + row_tok[t]) : n - 1;
+  auto masked_tile = [&](int j) {
+    if constexpr (MOD) return j * KT < lo_max || (j + 1) * KT > hi_min;
+    else return j >= j_mask;
+  };
+  // MOD: the bias of a row's head
+  [[maybe_unused]] float slope[RT];
+  if constexpr (MOD) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int rho = rho0 + 16 * RT * wave + 16 * t + col;
+      slope[t] = a.mod.slopes ? a.mod.slopes[kvh * G + min(rho, nrows - 1) % G] * kLog2e : 0.f;
+    }
+  }
 
   // Per-lane LDS byte offsets of the operand fragments inside a tile, recomputed where
   // they are used (a few VALU instructions; holding them would cost 12 registers).
@@ -847,22 +1016,29 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   float mx[RT];
   auto row_max = [&](int j, bool masked) __attribute__((always_inline)) {
     const int kt0 = j * KT;
+    if constexpr (MOD) {
+      int far[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) far[t] = base_pos + row_tok[t] - kt0 - 4 * grp;
+      modify_scores(sc, a.mod, a.scale_log2, slope, far);
+    }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       if (masked) {
         const int lim = limit[t] - kt0 - 4 * grp;  // keys 16 beta + r past it are out
+        [[maybe_unused]] const int low = MOD ? mfirst[t] - kt0 - 4 * grp : 0;  // and before it
 #pragma unroll
         for (int beta = 0; beta < NBETA; ++beta)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (16 * beta + r > lim) sc[t][beta][r] = -INFINITY;
+            if (16 * beta + r > lim || (MOD && 16 * beta + r < low)) sc[t][beta][r] = -INFINITY;
       }
       float x = -INFINITY;
 #pragma unroll
       for (int beta = 0; beta < NBETA; ++beta)
 #pragma unroll
         for (int r = 0; r < 4; ++r) x = fmaxf(x, sc[t][beta][r]);
-      mx[t] = score_rows_max(x) * a.scale_log2;
+      mx[t] = MOD ? score_rows_max(x) : score_rows_max(x) * a.scale_log2;
     }
   };
   auto softmax = [&](int j, bool masked) __attribute__((always_inline)) {
@@ -897,7 +1073,8 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
       for (int beta = 0; beta < NBETA; ++beta)
 #pragma unroll
         for (int r = 0; r < 4; ++r)  // probabilities replace the scores
-          sc[t][beta][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][beta][r], a.scale_log2, nref[t]));
+          sc[t][beta][r] = __builtin_amdgcn_exp2f(
+              MOD ? sc[t][beta][r] + nref[t] : __builtin_fmaf(sc[t][beta][r], a.scale_log2, nref[t]));
       // The P^T fragments of the first kPackedSteps 32-key steps are packed here (hi and
       // lo of step sg into score blocks 2 sg and 2 sg + 1); P.V packs the others.
 #pragma unroll
@@ -1002,7 +1179,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
     // after the softmax, by when the others' have drained.
     const bool late = wave >= 4 - PKV_PREFILL_LATE_DMA;  // wave-uniform
     if (!late) loads();
-    softmax(tbeg + m, tbeg + m >= j_mask);
+    softmax(tbeg + m, masked_tile(tbeg + m));
     if (late) loads();
 #if PKV_PREFILL_VALU_PRIO == 1
     __builtin_amdgcn_s_setprio(0);
@@ -1020,14 +1197,14 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   mfma_phase_begin();
   if (nt > 0) qk(0);
   mfma_phase_end();
-  if (PKV_PREFILL_EARLY_MAX && nt > 0) row_max(tbeg, tbeg >= j_mask);
+  if (PKV_PREFILL_EARLY_MAX && nt > 0) row_max(tbeg, masked_tile(tbeg));
   if (v_last >= 0) interval_v(0);
   for (int m = 1; m < nt; ++m) {
     open_m(m);
     mfma_phase_begin();
     pv_qk(m - 1, m);
     mfma_phase_end();
-    if (PKV_PREFILL_EARLY_MAX) row_max(tbeg + m, tbeg + m >= j_mask);
+    if (PKV_PREFILL_EARLY_MAX) row_max(tbeg + m, masked_tile(tbeg + m));
     interval_v(m);
   }
   for (int m = max(nt, 1); m <= ns; ++m) {
@@ -1083,9 +1260,19 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   }
 
   // O^T lane (row col, grp) holds dims 16 d + 4 grp + r of query row col.
+  [[maybe_unused]] uint32_t redo[RT];  // MOD: rows with a NaN
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const float l_tot = o[t][DTL][0];  // the whole row's sum, in every lane of its column
+    if constexpr (MOD) {
+      bool nan = false;
+#pragma unroll
+      for (int d = 0; d < DTL; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) nan = nan || !(fabsf(o[t][d][r]) < INFINITY);
+      const uint64_t b = __ballot(nan && row_ok[t]);
+      redo[t] = (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xFFFF);
+    }
     if (!row_ok[t]) continue;
     const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
     const int rho = rho0 + 16 * RT * wave + 16 * t + col;
@@ -1105,6 +1292,17 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
                        (uint32_t)Elt<DT>::from_f32(v4[2]) | ((uint32_t)Elt<DT>::from_f32(v4[3]) << 16));
       }
     }
+  }
+  if constexpr (MOD) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      for (; redo[t]; redo[t] &= redo[t] - 1) {
+        const int lr = __builtin_ctz(redo[t]);  // lane lr holds the row (and + 16, 32, 48)
+        const int rho = rho0 + 16 * RT * wave + 16 * t + lr;
+        redo_row<DT, HD>(a, it, rho / G, rho % G, __builtin_amdgcn_readlane(row_out[t], lr),
+                         __builtin_amdgcn_readlane(mfirst[t], lr), __builtin_amdgcn_readlane(mlast[t], lr),
+                         jbeg * KT, min(n, (jbeg + ntiles) * KT));
+      }
   }
 }
 
@@ -1146,10 +1344,10 @@ __device__ __forceinline__ PrefillItem pick_item(const PrefillArgs& a, const int
 }
 
 // Item `item` (chunk, row block, KV head): prefill_body at its coordinates.
-template <int DT, int HD, bool POW2, bool V16, bool ROWS>
+template <int DT, int HD, bool POW2, bool V16, bool ROWS, bool MOD = false>
 __device__ __forceinline__ void prefill_item(const PrefillArgs& a, const int item,
                                              PrefillLds<HD>& lds) {
-  prefill_body<DT, HD, POW2, V16, ROWS>(a, pick_item(a, item), lds);
+  prefill_body<DT, HD, POW2, V16, ROWS, MOD>(a, pick_item(a, item), lds);
 }
 
 // Head_dim 32 and 64 leave room for two workgroups on a CU (72 KB of LDS each at 64): the
@@ -1159,15 +1357,15 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& a, const int ite
 // them spills: fp16 at head_dim 64 with ROWS, 2 registers that the loop does not use. Looking
 // the rows of out up again at the end frees them and is not faster (76.3 us against 75.9 on
 // such chunks; at head_dim 128, where nothing spills, 131.7 against 129.4).
-template <int DT, int HD, bool V16> constexpr bool prefill_two_wgs() {
-  return HD <= 64 && (DT != PKV_BF16 || V16);
+template <int DT, int HD, bool V16, bool MOD> constexpr bool prefill_two_wgs() {
+  return HD <= 64 && (DT != PKV_BF16 || V16) && !MOD;
 }
 
-template <int DT, int HD, bool POW2, bool V16, bool ROWS>
-__global__ void __launch_bounds__(512, (prefill_two_wgs<DT, HD, V16>()) ? 4 : 2)
+template <int DT, int HD, bool POW2, bool V16, bool ROWS, bool MOD = false>
+__global__ void __launch_bounds__(512, (prefill_two_wgs<DT, HD, V16, MOD>()) ? 4 : 2)
 paged_prefill_kernel(const PrefillArgs a) {
   __shared__ __align__(16) PrefillLds<HD> lds;
-  prefill_item<DT, HD, POW2, V16, ROWS>(a, (int)blockIdx.x, lds);
+  prefill_item<DT, HD, POW2, V16, ROWS, MOD>(a, (int)blockIdx.x, lds);
 }
 
 // The fp16 copy of the chunks' V for the bf16 matrix-core prefill (PrefillArgs::v16):

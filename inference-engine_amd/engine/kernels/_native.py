@@ -7,6 +7,7 @@ dependency resolves to the HIP runtime torch has already loaded.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -146,6 +147,49 @@ SIGNATURES: dict[str, tuple] = {
          _i32, _i32, _i32, _i32, _f32,            # nh, nkv, hd, bs, scale
          _p, _i64, _p, _i64, _i64, _p],           # workspace, bytes, rows, len, num_rows, stream
     ),  # fmt: skip
+    "pkv_decode_mod_default_workgroups": (
+        _i32, [ctypes.c_int, _i32, _i32, _i32, _i32, _i32, _i32],
+    ),  # fmt: skip
+    "pkv_paged_decode_mod": (
+        ctypes.c_int,
+        [_p, ctypes.c_int, _i64, _i64,            # out
+         _p, _i64, _i64,                          # q
+         _p, _p, ctypes.c_int, _i64, _i64, _i64,  # k, v caches
+         _p, _i64, _i32,                          # block tables
+         _p, _i32, _i32, _i32, _i32, _i32,        # ctx, batch, nh, nkv, hd, bs
+         _f32, _i32, _p, _i64,                    # scale, wgs, workspace
+         _p, _i64,                                # rows, num_rows
+         _f32, _p, _p, _i64, _p, _p],             # softcap, slopes, ranges, stride, lse, stream
+    ),  # fmt: skip
+    "pkv_paged_prefill_mod": (
+        ctypes.c_int,
+        [_p, ctypes.c_int, _i64, _i64,            # out
+         _p, _i64, _i64,                          # q
+         _p, _p, ctypes.c_int, _i64, _i64, _i64,  # k, v caches
+         _p, _i64, _i32,                          # block tables
+         _p, _p, _i32, _i32,                      # ctx, cu_q, n_chunks, max_query_len
+         _i32, _i32, _i32, _i32, _f32,            # nh, nkv, hd, bs, scale
+         _p, _i64, _p, _i64, _i64,                # workspace, bytes, rows, len, num_rows
+         _f32, _p, _p, _i64, _p, _p],             # softcap, slopes, ranges, stride, lse, stream
+    ),  # fmt: skip
+    "pkv_attention_weights": (
+        ctypes.c_int,
+        [_p, _i64, _i64, _p, _f32,                # weights, stride, rows, row index, decay
+         _p, _i64, _i64,                          # q
+         _p, ctypes.c_int, _i64, _i64, _i64,      # k cache
+         _p, _i64, _i32,                          # block tables
+         _p, _p, _i32, _p,                        # ctx, cu_q, n_chunks, lse
+         _i32, _i32, _i32, _i32, _f32,            # nh, nkv, hd, bs, scale
+         _f32, _p, _p, _i64, _p],                 # softcap, slopes, ranges, stride, stream
+    ),  # fmt: skip
+    "pkv_evict_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "pkv_evict": (
+        ctypes.c_int,
+        [_p, _p, _i64, _i32, _i64, _i64,          # pools: layer stride, layers, row, slots
+         _p, _i64, _i64, _i64, _p,                # weights: strides, rows, row index
+         _p, _i64, _i32, _i32, _p, _i32,          # tables, stride, width, bs, ctx, batch
+         _i32, _i32, _p, _p, _i64, _p],           # keep, recent, new_lens, workspace, stream
+    ),  # fmt: skip
 }
 
 _lib: ctypes.CDLL | None = None
@@ -203,6 +247,14 @@ def stream_of(device: torch.device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def device_guard(device: torch.device):
+    """``device`` as the current one while the library is called (it asks the current device for
+    its CUs); nothing where it is already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 # Opt-in checks of step metadata. The kernels never fault on bad metadata: the append

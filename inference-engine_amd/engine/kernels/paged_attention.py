@@ -88,16 +88,20 @@ def decode_workgroups(device: torch.device, dtype: torch.dtype, head_dim: int,
 
 def default_workgroups(device: torch.device, dtype: torch.dtype, head_dim: int,
                        num_heads: int, num_kv_heads: int, batch: int, max_blocks: int,
-                       block_size: int) -> int:  # fmt: skip
+                       block_size: int, modified: bool = False) -> int:  # fmt: skip
     """What a call with the default split runs: 0 for the one-kernel per-sequence split
     (small batches of 16-bit K/V at head_dim 64/128; no workspace), else the stream-K
-    workgroup count. Static shapes only (a graph captured with it stays valid)."""
+    workgroup count. Static shapes only (a graph captured with it stays valid).
+    ``modified``: of a call with modified scores or ``lse``."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    key = (idx, dtype, head_dim, num_heads, num_kv_heads, batch, max_blocks, block_size)
+    key = (idx, dtype, head_dim, num_heads, num_kv_heads, batch, max_blocks, block_size, modified)
     wgs = _default_plan.get(key)
     if wgs is None:
+        lib = _native.lib()
+        query = lib.pkv_decode_mod_default_workgroups if modified else \
+            lib.pkv_decode_default_workgroups  # fmt: skip
         with torch.cuda.device(idx):
-            wgs = _native.lib().pkv_decode_default_workgroups(
+            wgs = query(
                 _native.dtype_code(dtype, "default_workgroups"), head_dim, num_heads,
                 num_kv_heads, batch, max_blocks, block_size)  # fmt: skip
         _native.check(min(wgs, 0), "default_workgroups")
@@ -350,6 +354,10 @@ def paged_decode_attention(
     prefix_groups: PrefixGroups | None = None,
     prefix_workgroups: int | None = None,
     rows: torch.Tensor | None = None,
+    softcap: float | None = None,
+    alibi_slopes: torch.Tensor | None = None,
+    key_ranges: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """q: [B, nh, hd]; k_cache, v_cache: [num_slots, nkv, hd] (one layer);
     block_tables: [B, max_blocks] int32; context_lens: [B] int32 -> [B, nh, hd].
@@ -376,6 +384,16 @@ def paged_decode_attention(
     sequence b's are row ``rows[b]`` of both -- ``out[rows] = attention(q[rows])`` without the
     gather and the scatter (``rows_in_place`` says whether their layouts allow it; not with
     ``prefix_groups``). Rows that no sequence names keep what they hold.
+
+    Modified scores (not with ``prefix_groups``; the reference has none):
+    ``softcap``: scores become ``softcap * tanh(score / softcap)``. ``alibi_slopes`` (float32
+    [nh], finite): then ``alibi_slopes[h] * (distance in tokens from the query to the key)`` is
+    taken off. ``key_ranges`` (int32 [rows of q, 2]): the query in row r of q sees the keys
+    ``key_ranges[r, 0] <= p < key_ranges[r, 1]`` of its context and no others (a sliding window;
+    ``step_key_ranges`` builds them); a range without keys gives 0, and what lies outside a range
+    does not reach its row, NaN and infinities included. ``lse`` (float32 [B, nh], contiguous)
+    receives the log2 normalisers of the scores, for ``paged_attention_weights``, in the order
+    of the sequences.
     """
     del block_n
     what = "paged_decode_attention"
@@ -400,6 +418,9 @@ def paged_decode_attention(
     if b == 0:
         return out
 
+    mod = _score_mod(what, dev, q, b, softcap, alibi_slopes, key_ranges, lse)
+    if mod is not None and prefix_groups is not None:
+        raise ValueError(f"{what}: modified scores and prefix_groups do not go together")
     max_blocks = block_tables.shape[1]
     lib = _native.lib()
     cascade = prefix_groups is not None and dtype in (torch.bfloat16, torch.float16) \
@@ -411,7 +432,8 @@ def paged_decode_attention(
     wg_arg = 0 if num_workgroups is None else num_workgroups
     if num_workgroups is None:
         num_workgroups = decode_workgroups(dev, dtype, hd, nh, nkv) if cascade else \
-            default_workgroups(dev, dtype, hd, nh, nkv, b, max_blocks, block_size)  # fmt: skip
+            default_workgroups(dev, dtype, hd, nh, nkv, b, max_blocks, block_size,
+                               mod is not None)  # fmt: skip
     ws_bytes = _workspace_bytes(num_workgroups, b, nh, hd, cascade) if num_workgroups else 0
     ws = None
     if ws_bytes and workspace is not None:
@@ -445,6 +467,10 @@ def paged_decode_attention(
             pg.q_rows.data_ptr(), o_pre.data_ptr(), lse_pre.data_ptr(),
             pg.prefix_row.data_ptr(), pg.pieces, pg.members, pwg, _native.stream_of(dev),
         )  # fmt: skip
+    elif mod is not None:
+        with _native.device_guard(dev):
+            status = lib.pkv_paged_decode_mod(*common, None if rows is None else rows.data_ptr(),
+                                              n_rows, *mod, _native.stream_of(dev))  # fmt: skip
     elif rows is not None:
         status = lib.pkv_paged_decode_rows(*common, rows.data_ptr(), n_rows,
                                            _native.stream_of(dev))  # fmt: skip
@@ -453,6 +479,40 @@ def paged_decode_attention(
     if status:
         _native.check(status, what)
     return out
+
+
+def _score_mod(what: str, dev: torch.device, q: torch.Tensor, queries: int,
+               softcap: float | None, alibi_slopes: torch.Tensor | None,
+               key_ranges: torch.Tensor | None, lse: torch.Tensor | None) -> tuple | None:  # fmt: skip
+    """The C arguments of a call's modified scores and normalisers, checked; None when it has
+    neither."""
+    if softcap is None and alibi_slopes is None and key_ranges is None and lse is None:
+        return None
+    nh = q.shape[1]
+    cap = 0.0 if softcap is None else float(softcap)
+    if cap != 0.0 and not 1e-30 <= cap <= 1e30:
+        raise ValueError(f"{what}: softcap {softcap} must be positive and finite (0 or None: no cap)")
+    for name, x in (("alibi_slopes", alibi_slopes), ("key_ranges", key_ranges), ("lse", lse)):
+        if x is not None and x.device != dev:
+            raise ValueError(f"{what}: {name} must be on {dev}, got {x.device}")
+    if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or
+                                     alibi_slopes.shape != (nh,) or
+                                     not alibi_slopes.is_contiguous()):  # fmt: skip
+        raise ValueError(f"{what}: alibi_slopes must be a contiguous float32 [{nh}] tensor")
+    stride = 0
+    if key_ranges is not None:
+        if key_ranges.dtype != torch.int32:
+            raise TypeError(f"{what}: key_ranges must be int32")
+        if key_ranges.shape != (q.shape[0], 2) or key_ranges.stride(1) != 1:
+            raise ValueError(f"{what}: key_ranges must be [{q.shape[0]}, 2] (one row per row of q), "
+                             "unit stride in a row")  # fmt: skip
+        stride = key_ranges.stride(0)
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (queries, nh) or
+                            not lse.is_contiguous()):  # fmt: skip
+        raise ValueError(f"{what}: lse must be a contiguous float32 [{queries}, {nh}] tensor")
+    return (cap, None if alibi_slopes is None else alibi_slopes.data_ptr(),
+            None if key_ranges is None else key_ranges.data_ptr(), stride,
+            None if lse is None else lse.data_ptr())  # fmt: skip
 
 
 @functools.lru_cache(maxsize=1024)
@@ -642,6 +702,10 @@ def paged_prefill_attention(
     out: torch.Tensor | None = None,
     workspace: torch.Tensor | None = None,
     rows: torch.Tensor | None = None,
+    softcap: float | None = None,
+    alibi_slopes: torch.Tensor | None = None,
+    key_ranges: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Bottom-right causal attention of prompt chunks over the paged pool.
 
@@ -665,6 +729,10 @@ def paged_prefill_attention(
     size through torch (at most ``PREFILL_WORKSPACE_MAX_BYTES``; beyond it, and for other
     dtypes, the call takes no copy). ``rows`` (int64 [T], with ``out``): token t's query is row
     ``rows[t]`` of q and its result goes to that row of out, as in ``paged_decode_attention``.
+    ``softcap``, ``alibi_slopes``, ``key_ranges`` (one row per row of q, instead of the causal
+    limit: windows, documents that do not see each other, prefixes that see themselves both ways)
+    and ``lse`` (float32 [T, nh] in the order of the query tokens): modified scores and normalisers,
+    as in ``paged_decode_attention``; query i of a chunk sits at position ctx_c - q_c + i.
     """
     what = "paged_prefill_attention"
     dev = _native.require_gpu(what, q, k_cache, v_cache, block_tables, context_lens,
@@ -702,6 +770,7 @@ def paged_prefill_attention(
         raise ValueError(f"{what}: out must be [T, nh, hd] of {q.dtype} or float32 on {dev}")
     if block_size <= 0:
         raise ValueError(f"{what}: block_size must be positive")
+    mod = _score_mod(what, dev, q, t, softcap, alibi_slopes, key_ranges, lse)
     if n_chunks == 0 or t == 0:
         return out
     if _native.debug_checks():
@@ -732,7 +801,11 @@ def paged_prefill_attention(
         nh, nkv, hd, block_size, hd**-0.5, ws_ptr, ws_bytes,
     )  # fmt: skip
     lib = _native.lib()
-    if rows is None:
+    if mod is not None:
+        with _native.device_guard(dev):
+            status = lib.pkv_paged_prefill_mod(*args, None if rows is None else rows.data_ptr(), t,
+                                               q.shape[0], *mod, _native.stream_of(dev))  # fmt: skip
+    elif rows is None:
         status = lib.pkv_paged_prefill_ws(*args, _native.stream_of(dev))
     else:
         status = lib.pkv_paged_prefill_rows(*args, rows.data_ptr(), t, q.shape[0],
@@ -740,6 +813,116 @@ def paged_prefill_attention(
     if status:
         _native.check(status, what)
     return out
+
+
+def paged_attention_weights(
+    weights: torch.Tensor,
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    lse: torch.Tensor,
+    cu_seqlens_q: torch.Tensor | None = None,
+    max_query_len: int = 1,
+    *,
+    decay: float = 1.0,
+    weight_rows: torch.Tensor | None = None,
+    softcap: float | None = None,
+    alibi_slopes: torch.Tensor | None = None,
+    key_ranges: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Adds the attention weights of a step's queries to those of the steps before, in place:
+    ``weights[row, p] = decay * weights[row, p] + sum`` over a sequence's queries and all heads of
+    the softmax weight that each gives to the cached token at position p (what
+    ``evict_tokens`` chooses by). No counterpart in the reference, which evicts no token.
+
+    weights: float32 [R, >= W * block_size], unit stride along positions; sequence c's is row
+    ``weight_rows[c]`` (int64 [C]; None: c; a row outside [0, R): the sequence is skipped; distinct
+    rows). q, k_cache, block_tables [C, W], context_lens [C], block_size, cu_seqlens_q [C + 1] and
+    max_query_len as in ``paged_prefill_attention`` (cu_seqlens_q None: one query per sequence, as
+    in ``paged_decode_attention``); a prompt's chunk can give its last queries alone (they are the
+    last tokens of its context). lse: float32 [T, nh], contiguous, from the attention call over the
+    same keys with the same ``softcap``, ``alibi_slopes`` and ``key_ranges``. ``decay`` 0: what
+    weights held is not read. Positions at or past a sequence's context keep what they hold:
+    clear a row when a sequence takes it. Sums are fp32, in a fixed order. Returns weights.
+    """
+    what = "paged_attention_weights"
+    tensors = [weights, q, k_cache, block_tables, context_lens, lse]
+    tensors += [x for x in (cu_seqlens_q, weight_rows) if x is not None]
+    dev = _native.require_gpu(what, *tensors)
+    if q.dim() != 3 or k_cache.dim() != 3:
+        raise ValueError(f"{what}: q [T, nh, hd] and k_cache [slots, nkv, hd] expected")
+    t, nh, hd = q.shape
+    nkv = k_cache.shape[1]
+    if k_cache.shape[2] != hd or nkv == 0 or nh == 0 or nh % nkv:
+        raise ValueError(f"{what}: cache {tuple(k_cache.shape)} does not fit q {tuple(q.shape)}")
+    if hd not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"{what}: head_dim {hd} not in {SUPPORTED_HEAD_DIMS}")
+    if k_cache.dtype != q.dtype:
+        raise TypeError(f"{what}: q {q.dtype} and k_cache {k_cache.dtype} must share one dtype")
+    if k_cache.stride(2) != 1:
+        raise ValueError(f"{what}: k_cache needs unit stride in head_dim")
+    n = context_lens.numel()
+    for name, x in (("block_tables", block_tables), ("context_lens", context_lens),
+                    ("cu_seqlens_q", cu_seqlens_q)):  # fmt: skip
+        if x is not None and x.dtype != torch.int32:
+            raise TypeError(f"{what}: {name} must be int32")
+    if block_tables.dim() != 2 or block_tables.shape[0] != n or block_tables.stride(1) != 1 or \
+            context_lens.shape != (n,) or not context_lens.is_contiguous():  # fmt: skip
+        raise ValueError(f"{what}: block_tables [C, W] (unit column stride), context_lens [C]")
+    if block_size <= 0:
+        raise ValueError(f"{what}: block_size must be positive")
+    if cu_seqlens_q is None:
+        if t != n:
+            raise ValueError(f"{what}: {t} queries for {n} sequences without cu_seqlens_q")
+    elif cu_seqlens_q.shape != (n + 1,) or not cu_seqlens_q.is_contiguous():
+        raise ValueError(f"{what}: cu_seqlens_q must be a contiguous [C + 1] tensor")
+    if weights.dtype != torch.float32 or weights.dim() != 2 or weights.stride(1) != 1:
+        raise ValueError(f"{what}: weights must be a float32 [R, positions] tensor, unit stride "
+                         "along positions")  # fmt: skip
+    if weights.shape[1] < block_tables.shape[1] * block_size:
+        raise ValueError(f"{what}: weights rows of {weights.shape[1]} for tables of "
+                         f"{block_tables.shape[1]} x {block_size} tokens")  # fmt: skip
+    _check_weight_rows(what, weight_rows, n, weights.shape[0], weights.stride(0), weights.shape[1])
+    if not 0.0 <= decay < float("inf"):
+        raise ValueError(f"{what}: decay {decay} must be finite and not negative")
+    mod = _score_mod(what, dev, q, t, softcap, alibi_slopes, key_ranges, lse)
+    if n == 0:
+        return weights
+    if _native.debug_checks():
+        if cu_seqlens_q is not None:
+            _check_chunks(what, block_tables, context_lens, block_size, k_cache.shape[0],
+                          cu_seqlens_q, t, max_query_len)  # fmt: skip
+        else:
+            _native.check_tables(what, block_tables, context_lens, block_size, k_cache.shape[0])
+    q = q.contiguous()
+    with _native.device_guard(dev):
+        status = _native.lib().pkv_attention_weights(
+            weights.data_ptr(), weights.stride(0), weights.shape[0],
+            None if weight_rows is None else weight_rows.data_ptr(), float(decay),
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+            _native.dtype_code(q.dtype, what), k_cache.stride(0), k_cache.stride(1),
+            k_cache.shape[0], block_tables.data_ptr(), block_tables.stride(0),
+            block_tables.shape[1], context_lens.data_ptr(),
+            None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), n, lse.data_ptr(),
+            nh, nkv, hd, block_size, hd**-0.5, *mod[:4], _native.stream_of(dev))  # fmt: skip
+    if status:
+        _native.check(status, what)
+    return weights
+
+
+def _check_weight_rows(what: str, weight_rows: torch.Tensor | None, batch: int, rows: int,
+                       stride: int, width: int) -> None:  # fmt: skip
+    """One row of weights per sequence, rows that do not overlap."""
+    if rows > 1 and stride < width:
+        raise ValueError(f"{what}: rows of weights overlap (stride {stride}, {width} positions)")
+    if weight_rows is None:
+        if rows < batch:
+            raise ValueError(f"{what}: {rows} rows of weights for {batch} sequences")
+    elif weight_rows.dtype != torch.int64 or weight_rows.shape != (batch,) or \
+            not weight_rows.is_contiguous():  # fmt: skip
+        raise ValueError(f"{what}: weight_rows must be a contiguous int64 [{batch}] tensor")
 
 
 # Largest workspace paged_prefill_attention allocates by itself for the fp16 V copy.

@@ -153,6 +153,19 @@ class BlockManager:
         self.copies_total += len(pairs)
         return pairs
 
+    def shrink(self, seq_id: int, tokens: int) -> list[int]:
+        """Give back ``seq_id``'s blocks behind its first ``tokens`` tokens (after an eviction
+        cut it down); returns them. Shared ones only lose this holder."""
+        if tokens < 0:
+            raise ValueError(f"sequence {seq_id} cannot shrink to {tokens} tokens")
+        table = self.tables.get(seq_id, [])
+        keep = min(self._blocks_for(tokens), len(table))
+        dropped = table[keep:]
+        del table[keep:]
+        for block in dropped:
+            self.pool.release(block)
+        return dropped
+
     def free(self, seq_id: int) -> None:
         for block in self.tables.pop(seq_id, ()):
             self.pool.release(block)

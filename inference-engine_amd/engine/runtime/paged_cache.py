@@ -68,6 +68,14 @@ class PagedKVCache:
         block, engine/runtime/block_manager.py:130-150)."""
         copy_blocks(self.k, self.v, block_mapping, self.block_size)
 
+    def evict(self, weights: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+              keep: int, recent: int, *, weight_rows: torch.Tensor | None = None) -> torch.Tensor:  # fmt: skip
+        """Cut every sequence down to ``keep`` tokens in every layer (``evict_tokens`` on this
+        pool; weights: [layers, R, positions]). Returns the new context lengths, after which
+        ``BlockManager.shrink`` gives back the blocks behind them."""
+        return evict_tokens(self.k, self.v, weights, block_tables, context_lens, self.block_size,
+                            keep, recent, weight_rows=weight_rows)  # fmt: skip
+
 
 def kv_append(
     k_pool: torch.Tensor,
@@ -148,6 +156,175 @@ def copy_blocks(
         _native.stream_of(dev),
     )  # fmt: skip
     _native.check(status, what)
+
+
+def evict_tokens(
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    weights: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    keep: int,
+    recent: int,
+    *,
+    weight_rows: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Eviction by accumulated attention weight, in place (no counterpart in the reference,
+    which evicts no token). In every layer, a sequence of more than ``keep`` tokens keeps its last
+    ``recent`` and, of the others, the ``keep - recent`` with the largest weights (ties: the
+    earliest; a NaN counts as the smallest). The kept tokens' K and V rows move, in their order, to
+    the slots of positions 0 .. keep - 1, their weights likewise, and the weights of positions
+    keep .. n - 1 become 0. Layers choose for themselves; their new lengths agree:
+    int32 [B], min(n, keep) (``out``, which may be ``context_lens``, or a new tensor).
+
+    Pools [L, num_slots, nkv, hd], contiguous per layer (or one layer, 3-D); weights float32
+    [L, R, >= W * block_size] (or [R, ...] with 3-D pools), sequence b's in row ``weight_rows[b]``
+    (int64 [B]; None: b; outside [0, R): the sequence is left alone); block_tables int32 [B, W],
+    context_lens int32 [B]. Rows move in place, so an evicted sequence's blocks must be its own
+    (``BlockManager.prepare_write`` and ``copy_blocks`` first) and weight rows distinct; with the
+    debug checks on, a block that two tables name raises. Positions afterwards count kept tokens:
+    a bias by distance or a key range then measures in them. ``workspace`` (contiguous uint8 of
+    ``evict_workspace_bytes``) replaces the scratch otherwise taken from torch's allocator.
+    """
+    what = "evict_tokens"
+    tensors = [k_pool, v_pool, weights, block_tables, context_lens]
+    tensors += [x for x in (weight_rows, out, workspace) if x is not None]
+    dev = _native.require_gpu(what, *tensors)
+    if k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype or \
+            k_pool.stride() != v_pool.stride():  # fmt: skip
+        raise ValueError(f"{what}: K and V pools must match in shape, strides and dtype")
+    _native.dtype_code(k_pool.dtype, what)
+    if k_pool.dim() == 3:
+        k_pool, v_pool, weights = k_pool[None], v_pool[None], weights[None]
+    if k_pool.dim() != 4 or k_pool.numel() == 0 or \
+            not (k_pool[0].is_contiguous() and v_pool[0].is_contiguous()):  # fmt: skip
+        raise ValueError(f"{what}: pools must be [L, slots, nkv, hd], contiguous per layer")
+    layers, slots, nkv, hd = k_pool.shape
+    if layers > 1 and k_pool.stride(0) < slots * nkv * hd:
+        raise ValueError(f"{what}: layers overlap")
+    if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        raise TypeError(f"{what}: block_tables and context_lens must be int32")
+    b = context_lens.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != b or block_tables.stride(1) != 1 or \
+            context_lens.shape != (b,) or not context_lens.is_contiguous():  # fmt: skip
+        raise ValueError(f"{what}: block_tables [B, W] (unit column stride), context_lens [B]")
+    width = block_tables.shape[1]
+    if block_size <= 0 or slots % block_size:
+        raise ValueError(f"{what}: {slots} slots not a multiple of block_size {block_size}")
+    if not 0 <= recent <= keep:
+        raise ValueError(f"{what}: recent {recent} of keep {keep}")
+    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[0] != layers or \
+            weights.stride(2) != 1 or weights.shape[2] < width * block_size:  # fmt: skip
+        raise ValueError(f"{what}: weights must be float32 [{layers}, R, >= {width * block_size}], "
+                         "unit stride along positions")  # fmt: skip
+    if layers > 1 and weights.stride(0) < (weights.shape[1] - 1) * weights.stride(1) + weights.shape[2]:
+        raise ValueError(f"{what}: layers of weights overlap")
+    from engine.kernels.paged_attention import _check_weight_rows
+
+    _check_weight_rows(what, weight_rows, b, weights.shape[1], weights.stride(1), weights.shape[2])
+    if out is None:
+        out = torch.empty_like(context_lens)
+    elif out.dtype != torch.int32 or out.shape != (b,) or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be a contiguous int32 [B] tensor")
+    if b == 0:
+        return out
+    keep = min(int(keep), 0x7FFFFFFF)
+    recent = min(int(recent), keep)
+    if _native.debug_checks():
+        _native.check_tables(what, block_tables, context_lens, block_size, slots)
+        _check_own_blocks(what, block_tables, context_lens, block_size, keep, weight_rows,
+                          weights.shape[1])  # fmt: skip
+    lib = _native.lib()
+    need = lib.pkv_evict_workspace_bytes(layers, b, width, block_size, keep)
+    if need < 0:
+        _native.check(need, what)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.dtype != torch.uint8 or workspace.numel() < need or not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor of at least "
+                         f"{need} bytes")  # fmt: skip
+    elt = k_pool.element_size()
+    with _native.device_guard(dev):
+        status = lib.pkv_evict(
+            k_pool.data_ptr(), v_pool.data_ptr(), k_pool.stride(0) * elt, layers, nkv * hd * elt,
+            slots, weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[1],
+            None if weight_rows is None else weight_rows.data_ptr(), block_tables.data_ptr(),
+            block_tables.stride(0), width, block_size, context_lens.data_ptr(), b, keep, recent,
+            out.data_ptr(), workspace.data_ptr(), workspace.numel(), _native.stream_of(dev))  # fmt: skip
+    _native.check(status, what)
+    return out
+
+
+def evict_workspace_bytes(layers: int, batch: int, max_blocks: int, block_size: int, keep: int) -> int:
+    """Scratch of one ``evict_tokens`` call of these sizes, e.g. to allocate it outside a capture."""
+    n = _native.lib().pkv_evict_workspace_bytes(layers, batch, max_blocks, block_size,
+                                                min(keep, 0x7FFFFFFF))  # fmt: skip
+    if n < 0:
+        _native.check(n, "evict_workspace_bytes")
+    return int(n)
+
+
+def _check_own_blocks(what, block_tables, context_lens, block_size, keep, weight_rows, rows) -> None:
+    """IndexError where a block that an eviction moves tokens in stands twice in the tables."""
+    n = context_lens.long()[:, None]
+    used = torch.arange(block_tables.shape[1], device=n.device) * block_size < n
+    cut = (n > keep)[:, 0]
+    if weight_rows is not None:
+        cut &= (weight_rows >= 0) & (weight_rows < rows)
+    named = block_tables[used]
+    moved = block_tables[used & cut[:, None]]
+    ids, count = torch.unique(named, return_counts=True)
+    twice = torch.isin(moved, ids[count > 1])
+    if bool(twice.any()):
+        raise IndexError(f"{what}: blocks {moved[twice][:4].tolist()} of an evicted sequence stand "
+                         "in more than one place (copy-on-write first)")  # fmt: skip
+
+
+def step_key_ranges(
+    context_lens: Sequence[int],
+    query_lens: Sequence[int],
+    device: str | torch.device,
+    *,
+    window: int | None = None,
+    prefix_lens: Sequence[int] | None = None,
+    doc_starts: Sequence[Sequence[int]] | None = None,
+) -> torch.Tensor:
+    """``key_ranges`` of a step (int32 [N, 2], one row per new token in ``PagedBatch.build``'s
+    order): the token at position p sees the keys [first, last). By default [0, p + 1), cut by:
+    ``window``: the last ``window`` of them alone (itself included); ``doc_starts`` (per sequence,
+    ascending first positions of its documents): none before its own document's start. With
+    ``prefix_lens`` (per sequence) the tokens of the first prefix_lens[i] see each other both ways,
+    as far as the context holds them; window and documents still cut what lies before."""
+    if len(context_lens) != len(query_lens):
+        raise ValueError("step_key_ranges: one context and query length per sequence")
+    if window is not None and window < 1:
+        raise ValueError(f"step_key_ranges: window {window} must be positive")
+    for name, x in (("prefix_lens", prefix_lens), ("doc_starts", doc_starts)):
+        if x is not None and len(x) != len(context_lens):
+            raise ValueError(f"step_key_ranges: {name} needs one entry per sequence")
+    parts = []
+    for i, (ctx, q) in enumerate(zip(context_lens, query_lens, strict=True)):
+        if q < 0 or ctx < q:
+            raise ValueError(f"step_key_ranges: {q} new tokens in a context of {ctx}")
+        pos = torch.arange(ctx - q, ctx)
+        lo, hi = torch.zeros_like(pos), pos + 1
+        if window is not None:
+            lo = (hi - window).clamp(min=0)
+        if doc_starts is not None and len(doc_starts[i]):
+            starts = torch.tensor(list(doc_starts[i]))
+            if bool((starts[1:] < starts[:-1]).any()) or int(starts[0]) < 0:
+                raise ValueError("step_key_ranges: doc_starts must ascend from 0 or more")
+            own = torch.searchsorted(starts, pos, right=True) - 1
+            lo = torch.maximum(lo, torch.where(own >= 0, starts[own.clamp(min=0)], 0))
+        if prefix_lens is not None:
+            n = min(int(prefix_lens[i]), ctx)
+            hi = torch.where(pos < n, torch.full_like(hi, n), hi)
+        parts.append(torch.stack([lo, hi], -1))
+    ranges = torch.cat(parts) if parts else torch.zeros(0, 2, dtype=torch.int64)
+    return ranges.to(torch.int32).to(device)
 
 
 def decode_slots(block_tables: torch.Tensor, context_lens: torch.Tensor, block_size: int,
