@@ -20,22 +20,22 @@ struct EvictArgs {
   int32_t max_blocks, bs, layers, batch, keep, recent;
   const int32_t* ctx;
   int32_t* new_ctx;
-  int2* head;   // [layers, batch]: first and one past the last token that moves
-  int2* moves;  // [layers, batch, keep]: (from, to) slots of kept token i, -1 outside the pool
-  int32_t keep_stride;
+  int2* head;     // [layers, batch]: first and one past the last token that moves
+  int32_t* from;  // [layers, batch, keep]: slot that kept token i comes from, -1 outside the pool
+  int32_t keep_stride, bs_shift;
 };
 
 // ---------------------------------------------------------------------------------
 // Selection: one workgroup of 1,024 threads per (layer, sequence).
 //
 // Of the first n - recent tokens the k = keep - recent heaviest stay, ties by the lowest index.
-// Weights become unsigned keys in their order (NaN below all); the k-th largest key is built two
-// bits at a time from the top, each time by counting the keys at or above three candidates:
-// compares and scalar bit counts on keys in registers, and one barrier, instead of a histogram whose
-// LDS atomics would collide (weights share few exponents). Then rounds of 1,024 tokens in index
-// order give every kept token its place by prefix counts, move its weight there and leave its slots
-// for the move pass. R: keys per thread in registers while they are counted (R = 0: more tokens
-// than that, read from L2 in every counting round).
+// Weights become unsigned keys in their order (NaN below all); the k-th largest key is found eight
+// bits at a time from the top: a histogram in LDS of the digit of the keys that share the digits found
+// so far, and a suffix sum over its 256 bins by one wave. (Two bits at a time by counting compares, in
+// registers, took 16 rounds of all 16 waves: 20 us for 2,112 tokens, now 8.) Then rounds of 1,024
+// tokens in index order give every kept token its place by prefix counts, move its weight there and
+// leave its slot for the move pass. R: keys per thread in registers (R = 0: more tokens than that,
+// read from L2 in every pass).
 // ---------------------------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t weight_key(float x) {
@@ -44,12 +44,35 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
+// Sum over the 16 lanes of a row of lanes, in every one of them.
+__device__ __forceinline__ int row_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, kQuadXor1, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kQuadXor2, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kRowHalfMirror, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kRowMirror, 0xF, 0xF, false);
+  return x;
+}
+
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / kWave;
 
+// Inclusive prefix sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 to rows 2 and 3
+  return x;
+}
+
 template <int R>
-__global__ void __launch_bounds__(kSelThreads)
+__global__ void __launch_bounds__(kSelThreads, (R <= 4 ? 8 : 4))
 evict_select_kernel(const EvictArgs a) {
-  __shared__ int counts[2][kSelWaves][4];
+  static_assert(kSelWaves == 16, "a row of lanes holds the waves' counts");
+  __shared__ __align__(16) int hist[2][256];
+  __shared__ __align__(16) int2 counts[2][kSelWaves];
+  __shared__ int2 found;  // the digit, and the keys above it
   __shared__ int first_gap;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -81,81 +104,76 @@ evict_select_kernel(const EvictArgs a) {
     for (int j = 0; j < R; ++j) key[j] = weight_key(x[j]);
   }
   if (tid == 0) first_gap = n;
+  if (tid < 256) hist[0][tid] = 0;
 
-  // The largest key t with at least k keys >= t among the old tokens (k > 0).
+  // The k-th largest key t of the old tokens (k > 0), and how many of them are above it.
   uint32_t t = 0;
-  int above = 0;  // keys >= t + (the unit of the last two bits decided): in the end keys > t
-  if (k > 0) {
-    for (int bit = 30; bit >= 0; bit -= 2) {
-      const uint32_t c1 = t | (1u << bit), c2 = t | (2u << bit), c3 = t | (3u << bit);
-      int n1 = 0, n2 = 0, n3 = 0;
-      auto count = [&](int i, uint32_t kk) __attribute__((always_inline)) {
-        const bool in = i < old;
-        n1 += __popcll(__ballot(in && kk >= c1));
-        n2 += __popcll(__ballot(in && kk >= c2));
-        n3 += __popcll(__ballot(in && kk >= c3));
-      };
-      if constexpr (R > 0) {
+  int above = 0;
+  for (int pass = 0; k > 0 && pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    int* const h = hist[pass & 1];
+    __syncthreads();  // the histogram is clear; the last pass's digit has been read
+    auto count = [&](int i, uint32_t kk) __attribute__((always_inline)) {
+      if (i < old && (pass == 0 || (kk >> (shift + 8)) == t)) atomicAdd(&h[(kk >> shift) & 255u], 1);
+    };
+    if constexpr (R > 0) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) count(j * kSelThreads + tid, key[j]);
-      } else {
-        for (int j = 0; j < rounds; ++j) {
-          const int i = j * kSelThreads + tid;
-          count(i, i < old ? weight_key(w[i]) : 0u);
-        }
+      for (int j = 0; j < R; ++j) count(j * kSelThreads + tid, key[j]);
+    } else {
+      for (int j = 0; j < rounds; ++j) {
+        const int i = j * kSelThreads + tid;
+        count(i, i < old ? weight_key(w[i]) : 0u);
       }
-      int(*cnt)[4] = counts[(bit >> 1) & 1];  // two buffers: one barrier a round
-      if (lane == 0) {
-        cnt[wave][0] = n1;
-        cnt[wave][1] = n2;
-        cnt[wave][2] = n3;
-      }
-      __syncthreads();
-      int m1 = 0, m2 = 0, m3 = 0;
-#pragma unroll
-      for (int s = 0; s < kSelWaves; ++s) {
-        m1 += cnt[s][0];
-        m2 += cnt[s][1];
-        m3 += cnt[s][2];
-      }
-      // at(t) >= k holds; t grows to the largest candidate for which it still does
-      if (m3 >= k) t = c3;
-      else if (m2 >= k) t = c2, above = m3;
-      else if (m1 >= k) t = c1, above = m2;
-      else above = m1;
-      t = (uint32_t)__builtin_amdgcn_readfirstlane((int)t);
     }
+    __syncthreads();
+    if (wave == 0) {
+      // Lane l: bins 255 - 4 l down to 252 - 4 l; keys in them and in all higher bins.
+      const int4 c = *reinterpret_cast<const int4*>(&h[252 - 4 * lane]);
+      const int mine = c.x + c.y + c.z + c.w;
+      const int upto = wave_scan(mine) + above;
+      const uint64_t hit = __ballot(upto >= k);  // not empty: all of the prefix's keys and those above
+      if (lane == __builtin_ctzll(hit)) {
+        int over = upto - mine, d = 255 - 4 * lane;
+        const int bins[4] = {c.w, c.z, c.y, c.x};
+#pragma unroll
+        for (int u = 0; u < 3; ++u)
+          if (over + bins[u] < k && d == 255 - 4 * lane - u) over += bins[u], --d;
+        found = make_int2(d, over);
+      }
+    } else if (wave < 5) {
+      hist[(pass & 1) ^ 1][tid - kWave] = 0;
+    }
+    __syncthreads();
+    const int2 f = found;
+    t = t << 8 | (uint32_t)f.x;
+    above = f.y;
   }
   const int ties = k - above;  // tokens equal to t that stay, the first ones
 
   __syncthreads();
   const int32_t* trow = a.tables + (int64_t)b * a.table_stride;
   auto slot_of = [&](int p) {
-    const int id = trow[p / a.bs];
-    const int64_t sl = (int64_t)id * a.bs + p % a.bs;
+    const int blk = a.bs_shift >= 0 ? p >> a.bs_shift : p / a.bs, id = trow[blk];
+    const int64_t sl = (int64_t)id * a.bs + (p - blk * a.bs);
     return id >= 0 && sl < a.num_slots ? (int)sl : -1;  // num_slots < 2^31 (launch)
   };
-  int2* moves = a.moves + ((int64_t)layer * a.batch + b) * a.keep_stride;
+  int32_t* from = a.from + ((int64_t)layer * a.batch + b) * a.keep_stride;
   int before = 0, eq_before = 0;  // tokens kept for sure, and tokens equal to t, in earlier rounds
   auto emit = [&](int j, float xv, uint32_t kk) __attribute__((always_inline)) {
     const int i = j * kSelThreads + tid;
+    const int slot = i < n ? slot_of(i) : -1;
     const bool sure = (i < old && k > 0 && kk > t) || (i >= old && i < n);
     const bool eq = i < old && k > 0 && kk == t;
     const uint64_t bs = __ballot(sure), be = __ballot(eq);
-    int(*cnt)[4] = counts[j & 1];
-    if (lane == 0) {
-      cnt[wave][0] = __popcll(bs);
-      cnt[wave][1] = __popcll(be);
-    }
+    int2* const cnt = counts[j & 1];
+    if (lane == 0) cnt[wave] = make_int2(__popcll(bs), __popcll(be));
     __syncthreads();  // the round's weights are in registers; the earlier rounds' moves may be overtaken
-    int sb = before, eb = eq_before, st = 0, et = 0;
-#pragma unroll
-    for (int s = 0; s < kSelWaves; ++s) {
-      const int cs = cnt[s][0], ce = cnt[s][1];
-      if (s < wave) sb += cs, eb += ce;
-      st += cs;
-      et += ce;
-    }
+    const int2 c = cnt[lane & 15];
+    const bool prior = (lane & 15) < wave;
+    int sb = before + __builtin_amdgcn_readfirstlane(row_sum(prior ? c.x : 0));
+    int eb = eq_before + __builtin_amdgcn_readfirstlane(row_sum(prior ? c.y : 0));
+    const int st = __builtin_amdgcn_readfirstlane(row_sum(c.x));
+    const int et = __builtin_amdgcn_readfirstlane(row_sum(c.y));
     const uint64_t below = (1ull << lane) - 1;
     sb += __popcll(bs & below);
     eb += __popcll(be & below);
@@ -163,10 +181,10 @@ evict_select_kernel(const EvictArgs a) {
     const bool kept = sure || (eq && eb < ties);
     if (kept) {
       w[pos] = xv;
-      moves[pos] = make_int2(slot_of(i), slot_of(pos));
-    } else if (i < n) {
-      atomicMin(&first_gap, i);
+      from[pos] = slot;
     }
+    const uint64_t gone = __ballot(!kept && i < n);
+    if (gone && lane == 0) atomicMin(&first_gap, j * kSelThreads + wave * kWave + __builtin_ctzll(gone));
     before += st;
     eq_before += et;
   };
@@ -217,21 +235,23 @@ evict_move_kernel(const EvictArgs a, int slices) {
   const bool on = at < a.row_bytes;  // the last slice may be narrower
   if (!on) at = 0;
   char* pool = (part / slices ? a.v : a.k) + (seq / a.batch) * a.layer_bytes + at;
-  const int2* moves = a.moves + seq * a.keep_stride;
+  const int32_t* from = a.from + seq * a.keep_stride;
+  const int32_t* trow = a.tables + (seq % a.batch) * a.table_stride;
   const int r = lane / LPR;
 
-  // Loads go out without conditions (a token past the end, a slot outside the pool and a lane past
-  // the row read slot 0), so that the wait for one batch does not wait for the next.
+  // Loads go out without conditions (a token past the end reads the last one's, a slot outside the
+  // pool and a lane past the row slot 0), so that the wait for one batch does not wait for the next;
+  // where a token goes is worked out only when its row is written.
   struct Moves {
-    int from[U], to[U];
+    int from[U], id[U];
   };
+  auto blk_of = [&](int i) { return a.bs_shift >= 0 ? i >> a.bs_shift : i / a.bs; };
   auto load_moves = [&](int i0, Moves& m) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * RPL + r;
-      const int2 p = moves[min(i, h.y - 1)];
-      m.from[u] = p.x;
-      m.to[u] = i < h.y && p.x >= 0 ? p.y : -1;
+      const int i = min(i0 + u * RPL + r, h.y - 1);
+      m.from[u] = from[i];
+      m.id[u] = trow[blk_of(i)];
     }
   };
   auto load_rows = [&](const Moves& m, u32x4* d) __attribute__((always_inline)) {
@@ -253,13 +273,25 @@ evict_move_kernel(const EvictArgs a, int slices) {
     __asm__ volatile("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]),
                           "+v"(x[6]), "+v"(x[7]) : : "memory");
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (on && cur.to[u] >= 0) *reinterpret_cast<u32x4*>(pool + (int64_t)cur.to[u] * a.row_bytes) = x[u];
+    for (int u = 0; u < U; ++u) {
+      const int p = i + u * RPL + r;
+      const int64_t to = (int64_t)cur.id[u] * a.bs + (p - blk_of(p) * a.bs);
+      if (on && p < h.y && cur.from[u] >= 0 && cur.id[u] >= 0 && to < a.num_slots)
+        *reinterpret_cast<u32x4*>(pool + to * a.row_bytes) = x[u];
+    }
     cur = next;
     next = after;
 #pragma unroll
     for (int u = 0; u < U; ++u) x[u] = nx[u];
   }
+}
+
+template <int SLICE> int launch_move(const EvictArgs& a, int64_t seqs, hipStream_t st) {
+  const int64_t slices = (a.row_bytes + SLICE - 1) / SLICE;
+  const int64_t wgs = (seqs * 2 * slices + 3) / 4;
+  if (slices > (1 << 20) || wgs >= ((int64_t)1 << 24)) return PKV_E_SHAPE;
+  hipLaunchKernelGGL(evict_move_kernel<SLICE>, dim3((unsigned)wgs), dim3(256), 0, st, a, (int)slices);
+  return (int)hipGetLastError();
 }
 
 struct EvictWs {
@@ -268,7 +300,7 @@ struct EvictWs {
 EvictWs evict_ws(int32_t layers, int32_t batch, int32_t keep) {
   const int64_t pairs = (int64_t)layers * batch;
   const int64_t moves = (pairs * 8 + 255) / 256 * 256;
-  return {moves, moves + pairs * keep * 8};
+  return {moves, moves + pairs * keep * 4};
 }
 
 }  // namespace
@@ -330,7 +362,8 @@ int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride_bytes, int32_t la
   a.ctx = context_lens;
   a.new_ctx = new_lens;
   a.head = (int2*)workspace;
-  a.moves = (int2*)((char*)workspace + ws.moves);
+  a.from = (int32_t*)((char*)workspace + ws.moves);
+  a.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
   a.keep_stride = kept;
   hipStream_t st = (hipStream_t)stream;
   const int64_t seqs = (int64_t)layers * batch;
@@ -341,12 +374,15 @@ int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride_bytes, int32_t la
   else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || cap <= keep) return (int)e;
-  constexpr int SLICE = 64;
-  const int64_t slices = (row_bytes + SLICE - 1) / SLICE;
-  const int64_t wgs = (seqs * 2 * slices + 3) / 4;
-  if (slices > (1 << 20) || wgs >= ((int64_t)1 << 24)) return PKV_E_SHAPE;
-  hipLaunchKernelGGL(evict_move_kernel<SLICE>, dim3((unsigned)wgs), dim3(256), 0, st, a, (int)slices);
-  return (int)hipGetLastError();
+  // The widest slices that still make 16 waves per CU: 256 bytes keep a row's bytes together in
+  // memory (16 layers, 32 sequences down to 1,000 tokens of 1 KB rows, weights and all: 414 us, with 64
+  // bytes 552); where not even 64 make four per CU, 32 (16 layers, one sequence of 2,112 tokens down to
+  // 2,048: 35 us, with 64 bytes 38, with 256 143).
+  const int64_t pairs = seqs * 2;
+  if (pairs * ((row_bytes + 255) / 256) >= 4096) return launch_move<256>(a, seqs, st);
+  if (pairs * ((row_bytes + 127) / 128) >= 4096) return launch_move<128>(a, seqs, st);
+  if (pairs * ((row_bytes + 63) / 64) >= 1024) return launch_move<64>(a, seqs, st);
+  return launch_move<32>(a, seqs, st);
 }
 
 }  // extern "C"
