@@ -425,7 +425,8 @@ int pkv_paged_prefill_mod(void* out, int out_dtype, int64_t out_stride_tok, int6
 /*
  * Accumulated attention weights (no counterpart in the reference, which evicts no token). For
  * chunk c with query tokens cu_seqlens_q[c] .. cu_seqlens_q[c+1]-1 of q, last in its context of n_c
- * tokens (cu_seqlens_q NULL: one query per chunk, row c), and every p < n_c:
+ * tokens (cu_seqlens_q NULL: one query per chunk, row c; max_query_len bounds every chunk's queries,
+ * those past it give nothing), and every p < n_c:
  *   w[p] = decay * w[p] + sum over its queries t and all heads h that see p of
  *          2^(s(t, h, p) - lse[t, h]),
  * s in log2 units, i.e. the softmax weights of the attention call that wrote lse (fp32 [tokens,
@@ -442,11 +443,18 @@ int pkv_attention_weights(float* weights, int64_t weight_stride, int64_t num_wei
                           int kv_dtype, int64_t kv_stride_slot, int64_t kv_stride_head,
                           int64_t num_slots, const int32_t* block_tables, int64_t table_stride,
                           int32_t max_blocks, const int32_t* context_lens,
-                          const int32_t* cu_seqlens_q, int32_t n_chunks, const float* lse,
-                          int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                          const int32_t* cu_seqlens_q, int32_t n_chunks, int32_t max_query_len,
+                          const float* lse, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                           int32_t block_size, float scale, float softcap,
                           const float* alibi_slopes, const int32_t* key_ranges,
-                          int64_t range_stride, void* stream);
+                          int64_t range_stride, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/* Its workspace (4-byte aligned, any contents): 0 for chunks of at most 16 query rows per KV head
+ * (max_query_len * num_heads / num_kv_heads), else a float per KV head and token of the tables. */
+int64_t pkv_attention_weights_workspace_bytes(int32_t num_heads, int32_t num_kv_heads,
+                                              int32_t n_chunks, int32_t max_query_len,
+                                              int32_t max_blocks, int32_t block_size);
 
 /*
  * Eviction by accumulated weight (no counterpart in the reference). In every layer l, sequence b of

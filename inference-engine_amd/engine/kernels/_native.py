@@ -178,10 +178,11 @@ SIGNATURES: dict[str, tuple] = {
          _p, _i64, _i64,                          # q
          _p, ctypes.c_int, _i64, _i64, _i64,      # k cache
          _p, _i64, _i32,                          # block tables
-         _p, _p, _i32, _p,                        # ctx, cu_q, n_chunks, lse
+         _p, _p, _i32, _i32, _p,                  # ctx, cu_q, n_chunks, max_query_len, lse
          _i32, _i32, _i32, _i32, _f32,            # nh, nkv, hd, bs, scale
-         _f32, _p, _p, _i64, _p],                 # softcap, slopes, ranges, stride, stream
+         _f32, _p, _p, _i64, _p, _i64, _p],       # softcap, slopes, ranges, stride, workspace, stream
     ),  # fmt: skip
+    "pkv_attention_weights_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "pkv_evict_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
     "pkv_evict": (
         ctypes.c_int,

@@ -831,6 +831,7 @@ def paged_attention_weights(
     softcap: float | None = None,
     alibi_slopes: torch.Tensor | None = None,
     key_ranges: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Adds the attention weights of a step's queries to those of the steps before, in place:
     ``weights[row, p] = decay * weights[row, p] + sum`` over a sequence's queries and all heads of
@@ -845,11 +846,13 @@ def paged_attention_weights(
     last tokens of its context). lse: float32 [T, nh], contiguous, from the attention call over the
     same keys with the same ``softcap``, ``alibi_slopes`` and ``key_ranges``. ``decay`` 0: what
     weights held is not read. Positions at or past a sequence's context keep what they hold:
-    clear a row when a sequence takes it. Sums are fp32, in a fixed order. Returns weights.
+    clear a row when a sequence takes it. Sums are fp32, in a fixed order. ``workspace`` (contiguous
+    uint8 of ``attention_weights_workspace_bytes``) replaces the scratch that calls of many queries
+    otherwise take from torch's allocator. Returns weights.
     """
     what = "paged_attention_weights"
     tensors = [weights, q, k_cache, block_tables, context_lens, lse]
-    tensors += [x for x in (cu_seqlens_q, weight_rows) if x is not None]
+    tensors += [x for x in (cu_seqlens_q, weight_rows, workspace) if x is not None]
     dev = _native.require_gpu(what, *tensors)
     if q.dim() != 3 or k_cache.dim() != 3:
         raise ValueError(f"{what}: q [T, nh, hd] and k_cache [slots, nkv, hd] expected")
@@ -897,6 +900,13 @@ def paged_attention_weights(
         else:
             _native.check_tables(what, block_tables, context_lens, block_size, k_cache.shape[0])
     q = q.contiguous()
+    queries = int(max_query_len) if cu_seqlens_q is not None else 1
+    need = attention_weights_workspace_bytes(nh, nkv, n, queries, block_tables.shape[1], block_size)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    elif workspace.dtype != torch.uint8 or workspace.numel() < need or not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be a contiguous uint8 tensor of at least "
+                         f"{need} bytes")  # fmt: skip
     with _native.device_guard(dev):
         status = _native.lib().pkv_attention_weights(
             weights.data_ptr(), weights.stride(0), weights.shape[0],
@@ -905,11 +915,25 @@ def paged_attention_weights(
             _native.dtype_code(q.dtype, what), k_cache.stride(0), k_cache.stride(1),
             k_cache.shape[0], block_tables.data_ptr(), block_tables.stride(0),
             block_tables.shape[1], context_lens.data_ptr(),
-            None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), n, lse.data_ptr(),
-            nh, nkv, hd, block_size, hd**-0.5, *mod[:4], _native.stream_of(dev))  # fmt: skip
+            None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), n, int(max_query_len),
+            lse.data_ptr(),
+            nh, nkv, hd, block_size, hd**-0.5, *mod[:4],
+            None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel(), _native.stream_of(dev))  # fmt: skip
     if status:
         _native.check(status, what)
     return weights
+
+
+@functools.lru_cache(maxsize=1024)
+def attention_weights_workspace_bytes(num_heads: int, num_kv_heads: int, n_chunks: int,
+                                      max_query_len: int, max_blocks: int, block_size: int) -> int:  # fmt: skip
+    """Scratch of one ``paged_attention_weights`` call of these static sizes (0 for few queries)."""
+    n = _native.lib().pkv_attention_weights_workspace_bytes(num_heads, num_kv_heads, n_chunks,
+                                                            max_query_len, max_blocks, block_size)  # fmt: skip
+    if n < 0:
+        _native.check(n, "attention_weights_workspace_bytes")
+    return int(n)
 
 
 def _check_weight_rows(what: str, weight_rows: torch.Tensor | None, batch: int, rows: int,

@@ -63,8 +63,9 @@ def test_prefill_entry(over, code):
 def weights_args(**over):
     a = {"w": P, "wst": 64, "wn": 2, "wr": None, "decay": 1.0, "q": P, "qst": 1024, "qsh": 128,
          "k": P, "kdt": 2, "kss": 256, "ksh": 128, "slots": 64, "tables": P, "ts": 4, "width": 4,
-         "ctx": P, "cu": None, "n": 2, "lse": P, "nh": 8, "nkv": 2, "hd": 128, "bs": 16,
-         "scale": 0.1, "cap": 0.0, "slopes": None, "ranges": None, "rs": 0, "stream": None}  # fmt: skip
+         "ctx": P, "cu": None, "n": 2, "maxq": 1, "lse": P, "nh": 8, "nkv": 2, "hd": 128, "bs": 16,
+         "scale": 0.1, "cap": 0.0, "slopes": None, "ranges": None, "rs": 0, "work": None,
+         "bytes": 0, "stream": None}  # fmt: skip
     assert set(over) <= set(a)
     a.update(over)
     return list(a.values())
@@ -75,7 +76,10 @@ def weights_args(**over):
     [({"decay": -0.5}, -2), ({"decay": float("nan")}, -2), ({"decay": float("inf")}, -2),
      ({"wn": 1}, -2), ({"cap": -1.0}, -2), ({"hd": 48}, -2), ({"nkv": 3}, -2), ({"kdt": 9}, -1),
      ({"lse": None}, -5), ({"w": None}, -5), ({"q": P + 2}, -3), ({"kss": 100}, -3),
-     ({"width": 1 << 27, "bs": 16}, -2), ({"n": 0}, 0), ({"width": 0}, 0)],
+     ({"width": 1 << 27, "bs": 16}, -2), ({"slots": 1 << 31}, -2),
+     ({"cu": P, "maxq": -1}, -2), ({"cu": P, "maxq": 5}, -4),
+     ({"cu": P, "maxq": 5, "work": P, "bytes": 2 * 2 * 64 * 4 - 1}, -4), ({"bytes": -1}, -4),
+     ({"work": P + 2, "bytes": 64}, -3), ({"n": 0}, 0), ({"width": 0}, 0)],
 )  # fmt: skip
 def test_weights_entry(over, code):
     assert _native.lib().pkv_attention_weights(*weights_args(**over)) == code
@@ -103,13 +107,18 @@ def test_evict_entry(over, code):
 
 def test_workspace_queries():
     lib = _native.lib()
-    assert lib.pkv_evict_workspace_bytes(2, 3, 10, 16, 50) == 256 + 2 * 3 * 50 * 8
+    assert lib.pkv_evict_workspace_bytes(2, 3, 10, 16, 50) == 256 + 2 * 3 * 50 * 4
     # no more moves than a table holds tokens
-    assert lib.pkv_evict_workspace_bytes(1, 1, 2, 16, 1 << 30) == 256 + 32 * 8
+    assert lib.pkv_evict_workspace_bytes(1, 1, 2, 16, 1 << 30) == 256 + 32 * 4
     assert lib.pkv_evict_workspace_bytes(1, 1, 2, 0, 4) == -2
-    assert evict_workspace_bytes(1, 1, 2, 16, 1 << 40) == 256 + 32 * 8
+    assert evict_workspace_bytes(1, 1, 2, 16, 1 << 40) == 256 + 32 * 4
     with pytest.raises(ValueError):
         evict_workspace_bytes(1, 1, 2, 16, -1)
+    assert lib.pkv_attention_weights_workspace_bytes(32, 8, 3, 4, 10, 16) == 0
+    assert lib.pkv_attention_weights_workspace_bytes(32, 8, 3, 5, 10, 16) == 3 * 8 * 160 * 4
+    assert lib.pkv_attention_weights_workspace_bytes(32, 5, 3, 5, 10, 16) == -2
+    with pytest.raises(ValueError):
+        pa.attention_weights_workspace_bytes(32, 8, -1, 5, 10, 16)
     assert lib.pkv_decode_mod_default_workgroups(2, 96, 24, 8, 8, 32, 16) == -2
     assert lib.pkv_decode_mod_default_workgroups(7, 128, 24, 8, 8, 32, 16) == -1
     assert ctypes.sizeof(ctypes.c_int64) == 8
