@@ -8,8 +8,7 @@
 
 namespace pkv {
 // prefill_mod.hip: the 16-bit matrix-core kernel with modified scores.
-hipError_t launch_prefill_mod(const PrefillArgs& a, int kv_dtype, int head_dim, int64_t rows,
-                              hipStream_t st);
+hipError_t launch_prefill_mod(PrefillArgs a, int kv_dtype, int head_dim, int64_t rows, hipStream_t st);
 }  // namespace pkv
 
 namespace {

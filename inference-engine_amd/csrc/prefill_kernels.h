@@ -45,7 +45,7 @@ struct PrefillArgs {
   // negative values count from the end, a row outside is skipped. Not with q_rows.
   const int64_t* rows;
   int64_t rows_len, num_rows;
-  ScoreMod mod;  // read by the kernels instantiated with MOD
+  ScoreMod mod;  // read by the kernels instantiated with a MOD
 };
 
 // Query token t's row of q and out through `rows` (non-null), or -1.
@@ -478,9 +478,20 @@ template <int HD> struct PrefillLds {
 // runs several items on one workgroup puts a barrier between them (the merge reuses the
 // rings).
 // ROWS: q and out rows through a.rows (else a.rows is null).
-// MOD: modified scores (a.mod), with ROWS, and a.rows may be null. Every query row then has its
-// own first and last key; the item's tiles run from the smallest to the largest of them.
-template <int DT, int HD, bool POW2, bool V16, bool ROWS, bool MOD = false>
+// MOD: which modified scores (a.mod), with ROWS, and a.rows may be null. Every query row then has
+// its own first and last key; the item's tiles run from the smallest to the largest of them.
+//   kModRanges: no cap, no bias.
+//   kModCap: a cap, no bias. Scores stay raw until the exponent, where the cap costs 3 multiply-adds
+//     each (a tile with a score past 0.3 of the cap: the exact form, an exp2 and a reciprocal).
+//   kModBias: a bias, no cap. It is what Q.K^T starts its sums from, so the softmax sees it as part of
+//     the raw score. Taken against the row's nearest key, whose bias the normaliser gets back: its
+//     rounding then matters only to weights that it makes small.
+//   kModAny: both, either or none.
+// One prompt of 6,011 tokens, 32 / 8 heads, head_dim 128, bf16, on a day when the plain kernel took
+// 303 us with the copy of V: ranges 314, cap 353 (412 where every tile takes the exact form), bias
+// 352, both 449. Bound by vector instructions: each one per score is some 20 us. (One kernel for all
+// of them that branched took 346, 452, 452, 422 and 523.)
+template <int DT, int HD, bool POW2, bool V16, bool ROWS, int MOD = 0>
 __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const PrefillItem& it,
                                              PrefillLds<HD>& lds) {
   using SH = PrefillShape<HD>;
@@ -566,7 +577,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       mfirst[t] = 0;
-      mlast[t] = a.causal ? min(n - 1, base_pos + row_tok[t]) : n - 1;
+      mlast[t] = a.causal ? max(min(n - 1, base_pos + row_tok[t]), -1) : n - 1;
     }
     hi_min = (a.causal ? min(n - 1, base_pos + rho0 / G) : n - 1) + 1;
     if (a.mod.ranges) {
@@ -814,23 +825,39 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   // past the smallest limit among this workgroup's rows (its first row's).
   const int limit_min = a.causal ? min(n - 1, base_pos + rho0 / G) : n - 1;
   const int j_mask = min(ntiles, max(0, (limit_min + 1) / KT));
-  int limit[RT];  // last key each of this lane's rows sees
+  [[maybe_unused]] int limit[RT];  // last key each of this lane's rows sees (MOD: mlast)
 #pragma unroll
   for (int t = 0; t < RT; ++t)
-    limit[t] = MOD ? mlast[t] : a.causal ? min(n - 1, base_pos + row_tok[t]) : n - 1;
+    limit[t] = a.causal ? min(n - 1, base_pos + row_tok[t]) : n - 1;
   auto masked_tile = [&](int j) {
     if constexpr (MOD) return j * KT < lo_max || (j + 1) * KT > hi_min;
     else return j >= j_mask;
   };
-  // MOD: the bias of a row's head
-  [[maybe_unused]] float slope[RT];
-  if constexpr (MOD) {
+  // The bias of a row's head, in log2 units (kModAny) or raw ones with the nearest key's (kModBias).
+  [[maybe_unused]] float slope[RT], nearest[RT];
+  if constexpr (MOD >= kModBias) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int rho = rho0 + 16 * RT * wave + 16 * t + col;
       slope[t] = a.mod.slopes ? a.mod.slopes[kvh * G + min(rho, nrows - 1) % G] * kLog2e : 0.f;
+      if constexpr (MOD == kModBias) {
+        slope[t] /= a.scale_log2;
+        const int pos = base_pos + row_tok[t];
+        nearest[t] = slope[t] * (float)max(max(pos - mlast[t], mfirst[t] - pos), 0);
+      }
     }
   }
+  // What Q.K^T of 16-key block beta of tile j starts from in row tile t.
+  auto score_start = [&](int j, int t, int beta) __attribute__((always_inline)) {
+    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (MOD == kModBias) {
+      const float far = (float)(base_pos + row_tok[t] - j * KT - 4 * grp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        c[r] = __builtin_fmaf(-slope[t], fabsf(far - (float)(16 * beta + r)), nearest[t]);
+    }
+    return c;
+  };
 
   // Per-lane LDS byte offsets of the operand fragments inside a tile, recomputed where
   // they are used (a few VALU instructions; holding them would cost 12 registers).
@@ -874,7 +901,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
     for (int beta = 0; beta < NBETA; ++beta) {
       if (beta) __builtin_amdgcn_sched_barrier(0);  // one 16-key block's K fragments at a time
 #pragma unroll
-      for (int t = 0; t < RT; ++t) sc[t][beta] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < RT; ++t) sc[t][beta] = score_start(tbeg + m, t, beta);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const u32x4 kf = *reinterpret_cast<const u32x4*>(stage + beta * 16 * CH * 16 +
@@ -994,7 +1021,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
         const int beta = ki(i) / KS, s = ki(i) % KS;
 #pragma unroll
         for (int t = 0; t < RT; ++t)
-          sc[t][beta] = MMA::mma(f, qf[t][s], s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sc[t][beta]);
+          sc[t][beta] = MMA::mma(f, qf[t][s], s == 0 ? score_start(tbeg + mq, t, beta) : sc[t][beta]);
       }
     };
     u32x4 buf[PIPE + 1];
@@ -1014,31 +1041,70 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   // The first part of the softmax of tile j: the causal mask and each row's maximum
   // (scaled to log2 units) into mx.
   float mx[RT];
+  [[maybe_unused]] bool past = false;  // kModCap: a score of the tile is past the series' range
   auto row_max = [&](int j, bool masked) __attribute__((always_inline)) {
     const int kt0 = j * KT;
-    if constexpr (MOD) {
+    if constexpr (MOD == kModAny) {
       int far[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) far[t] = base_pos + row_tok[t] - kt0 - 4 * grp;
-      modify_scores(sc, a.mod, a.scale_log2, slope, far);
+      // (the series' registers would spill where two workgroups share a CU: 134 us became 148 on
+      // the chunks of prefill_two_wgs)
+      modify_scores<(HD >= 128)>(sc, a.mod, a.scale_log2, slope, far);
+    }
+    // kModCap: the largest |s| that the lane has of each row bounds its maximum, which is looked for
+    // only where it could raise the reference.
+    bool look = true;
+    if constexpr (MOD == kModCap) {
+      bool over = false, high = false;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        float x = 0.f;
+#pragma unroll
+        for (int beta = 0; beta < NBETA; ++beta)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x = fmaxf(x, fabsf(sc[t][beta][r]));
+        over = over || x > a.mod.series_max;
+        high = high || x * a.scale_log2 > m_run[t] + 8.f;
+      }
+      past = __builtin_amdgcn_ballot_w64(over) != 0;
+      look = __builtin_amdgcn_ballot_w64(high) != 0;
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       if (masked) {
-        const int lim = limit[t] - kt0 - 4 * grp;  // keys 16 beta + r past it are out
-        [[maybe_unused]] const int low = MOD ? mfirst[t] - kt0 - 4 * grp : 0;  // and before it
+        if constexpr (MOD) {
+          // One compare per key, a block's at a time: first <= key <= last as an unsigned distance from
+          // the first. (Two compares each, all 32 in flight, spilled scalar registers.)
+          const int low = mfirst[t] - kt0 - 4 * grp;
+          const uint32_t keys = (uint32_t)(mlast[t] - mfirst[t] + 1);
 #pragma unroll
-        for (int beta = 0; beta < NBETA; ++beta)
+          for (int beta = 0; beta < NBETA; ++beta) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (16 * beta + r > lim || (MOD && 16 * beta + r < low)) sc[t][beta][r] = -INFINITY;
+            for (int r = 0; r < 4; ++r)
+              sc[t][beta][r] = (uint32_t)(16 * beta + r - low) < keys ? sc[t][beta][r] : -INFINITY;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        } else {
+          const int lim = limit[t] - kt0 - 4 * grp;  // keys 16 beta + r past it are out
+#pragma unroll
+          for (int beta = 0; beta < NBETA; ++beta)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (16 * beta + r > lim) sc[t][beta][r] = -INFINITY;
+        }
       }
+      mx[t] = -INFINITY;
+      if (!look) continue;  // uniform
       float x = -INFINITY;
 #pragma unroll
       for (int beta = 0; beta < NBETA; ++beta)
 #pragma unroll
         for (int r = 0; r < 4; ++r) x = fmaxf(x, sc[t][beta][r]);
-      mx[t] = MOD ? score_rows_max(x) : score_rows_max(x) * a.scale_log2;
+      if constexpr (MOD == kModAny) mx[t] = score_rows_max(x);
+      else mx[t] = score_rows_max(x) * a.scale_log2;
+      if constexpr (MOD == kModCap)  // the cap is monotone
+        mx[t] = mx[t] == -INFINITY ? mx[t] : capped<false>(a.mod, mx[t]);
     }
   };
   auto softmax = [&](int j, bool masked) __attribute__((always_inline)) {
@@ -1067,26 +1133,49 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
         for (int d = 0; d <= DTL; ++d) o[t][d] *= alpha;
       }
     }
+    // exponent(score, nref): less the row's reference
+    auto probabilities = [&](auto exponent) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
+      for (int t = 0; t < RT; ++t) {
 #pragma unroll
-      for (int beta = 0; beta < NBETA; ++beta)
+        for (int beta = 0; beta < NBETA; ++beta)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)  // probabilities replace the scores
-          sc[t][beta][r] = __builtin_amdgcn_exp2f(
-              MOD ? sc[t][beta][r] + nref[t] : __builtin_fmaf(sc[t][beta][r], a.scale_log2, nref[t]));
-      // The P^T fragments of the first kPackedSteps 32-key steps are packed here (hi and
-      // lo of step sg into score blocks 2 sg and 2 sg + 1); P.V packs the others.
+          for (int r = 0; r < 4; ++r)  // probabilities replace the scores
+            sc[t][beta][r] = __builtin_amdgcn_exp2f(exponent(sc[t][beta][r], nref[t]));
+        // The P^T fragments of the first kPackedSteps 32-key steps are packed here (hi and
+        // lo of step sg into score blocks 2 sg and 2 sg + 1); P.V packs the others.
 #pragma unroll
-      for (int sg = 0; sg < kPackedSteps; ++sg) {
-        float p8[8];
+        for (int sg = 0; sg < kPackedSteps; ++sg) {
+          float p8[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p8[e] = sc[t][2 * sg + e / 4][e % 4];
-        u32x4 hi, lo;
-        PM::pack8(p8, hi, lo);
-        sc[t][2 * sg] = __builtin_bit_cast(f32x4, hi);
-        sc[t][2 * sg + 1] = __builtin_bit_cast(f32x4, lo);
+          for (int e = 0; e < 8; ++e) p8[e] = sc[t][2 * sg + e / 4][e % 4];
+          u32x4 hi, lo;
+          PM::pack8(p8, hi, lo);
+          sc[t][2 * sg] = __builtin_bit_cast(f32x4, hi);
+          sc[t][2 * sg + 1] = __builtin_bit_cast(f32x4, lo);
+        }
       }
+    };
+    if constexpr (MOD == kModCap) {
+      // -inf (masked) stays -inf: the polynomial's last coefficient is positive; the exact form, which
+      // would saturate, gets 2^-100 of the score added.
+      if (past) {
+        const float c1 = a.mod.c1 * a.scale_log2, c2 = -2.f * a.mod.c2;
+        probabilities([&](float x, float ref) {
+          const float y = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c1));
+          return __builtin_fmaf(x, 0x1p-100f, __builtin_fmaf(c2, y, a.mod.c2 + ref));
+        });
+      } else {
+        probabilities([&](float x, float ref) {
+          const float y = x * x;
+          const float p = __builtin_fmaf(y, __builtin_fmaf(y, a.mod.series[1], a.mod.series[0]), a.scale_log2);
+          return __builtin_fmaf(x, p, ref);
+        });
+      }
+    } else if constexpr (MOD == kModAny) {
+      probabilities([&](float x, float ref) { return x + ref; });
+    } else {
+      probabilities([&](float x, float ref) { return __builtin_fmaf(x, a.scale_log2, ref); });
     }
   };
 
@@ -1276,9 +1365,10 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
     if (!row_ok[t]) continue;
     const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
     const int rho = rho0 + 16 * RT * wave + 16 * t + col;
+    const float far_bias = MOD == kModBias ? nearest[t] * a.scale_log2 : 0.f;
     if (a.lse && grp == 0)  // log2 normaliser: the exponent reference m_run plus log2(sum)
       a.lse[(int64_t)(q0 + rho / G) * a.nh + kvh * G + rho % G] =
-          l_tot > 0.f ? m_run[t] + (__log2f(l_tot) - PM::kPLog2) : -INFINITY;
+          l_tot > 0.f ? m_run[t] + (__log2f(l_tot) - PM::kPLog2) - far_bias : -INFINITY;
     const int64_t e0 = (ROWS ? (int64_t)row_out[t] : (int64_t)(q0 + rho / G)) * a.out_st + (int64_t)(kvh * G + rho % G) * a.out_sh;
 #pragma unroll
     for (int d = 0; d < DTL; ++d) {
@@ -1344,7 +1434,7 @@ __device__ __forceinline__ PrefillItem pick_item(const PrefillArgs& a, const int
 }
 
 // Item `item` (chunk, row block, KV head): prefill_body at its coordinates.
-template <int DT, int HD, bool POW2, bool V16, bool ROWS, bool MOD = false>
+template <int DT, int HD, bool POW2, bool V16, bool ROWS, int MOD = 0>
 __device__ __forceinline__ void prefill_item(const PrefillArgs& a, const int item,
                                              PrefillLds<HD>& lds) {
   prefill_body<DT, HD, POW2, V16, ROWS, MOD>(a, pick_item(a, item), lds);
@@ -1356,12 +1446,15 @@ __device__ __forceinline__ void prefill_item(const PrefillArgs& a, const int ite
 // ones, 32 / 8 heads, 109.6 us per call, now 90.4; bf16 without the copy would spill 18). One of
 // them spills: fp16 at head_dim 64 with ROWS, 2 registers that the loop does not use. Looking
 // the rows of out up again at the end frees them and is not faster (76.3 us against 75.9 on
-// such chunks; at head_dim 128, where nothing spills, 131.7 against 129.4).
-template <int DT, int HD, bool V16, bool MOD> constexpr bool prefill_two_wgs() {
-  return HD <= 64 && (DT != PKV_BF16 || V16) && !MOD;
+// such chunks; at head_dim 128, where nothing spills, 131.7 against 129.4). Modified scores at
+// head_dim 64 spill 9 registers with ranges (fp16, those chunks with documents of 400 tokens: 51 us
+// with one workgroup per CU, 36 with two), 16-31 with a bias (135 and 109) and 31 with a cap alone,
+// which is faster with one (119 us, with two 136).
+template <int DT, int HD, bool V16, int MOD> constexpr bool prefill_two_wgs() {
+  return HD <= 64 && (DT != PKV_BF16 || V16) && !(MOD == kModCap && HD == 64);
 }
 
-template <int DT, int HD, bool POW2, bool V16, bool ROWS, bool MOD = false>
+template <int DT, int HD, bool POW2, bool V16, bool ROWS, int MOD = 0>
 __global__ void __launch_bounds__(512, (prefill_two_wgs<DT, HD, V16, MOD>()) ? 4 : 2)
 paged_prefill_kernel(const PrefillArgs a) {
   __shared__ __align__(16) PrefillLds<HD> lds;

@@ -14,10 +14,17 @@ template <int DT, int HD, bool V16> hipError_t launch_hd(PrefillArgs a, int64_t 
   const int64_t items = (int64_t)a.row_blocks * a.nkv * a.n_chunks;
   if (items > 0x7FFFFFFF) return hipErrorInvalidValue;
   const dim3 grid((unsigned)items), block(512);
-  if (a.bs_shift >= 0)
-    hipLaunchKernelGGL((paged_prefill_kernel<DT, HD, true, V16, true, true>), grid, block, 0, st, a);
-  else
-    hipLaunchKernelGGL((paged_prefill_kernel<DT, HD, false, V16, true, true>), grid, block, 0, st, a);
+  // Block sizes that are no power of two have the general kernel only.
+  const int mod = a.bs_shift < 0 ? 0 : a.mod.slopes ? (a.mod.c2 != 0.f ? kModAny : kModBias)
+                                                    : (a.mod.c2 != 0.f ? kModCap : kModRanges);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a); };
+  switch (mod) {
+    case kModRanges: go(paged_prefill_kernel<DT, HD, true, V16, true, kModRanges>); break;
+    case kModCap: go(paged_prefill_kernel<DT, HD, true, V16, true, kModCap>); break;
+    case kModBias: go(paged_prefill_kernel<DT, HD, true, V16, true, kModBias>); break;
+    case kModAny: go(paged_prefill_kernel<DT, HD, true, V16, true, kModAny>); break;
+    default: go(paged_prefill_kernel<DT, HD, false, V16, true, kModAny>);
+  }
   return hipGetLastError();
 }
 
@@ -35,8 +42,8 @@ hipError_t launch(const PrefillArgs& a, int hd, int64_t rows, hipStream_t st) {
 
 namespace pkv {
 
-hipError_t launch_prefill_mod(const PrefillArgs& a, int kv_dtype, int head_dim, int64_t rows,
-                              hipStream_t st) {
+hipError_t launch_prefill_mod(PrefillArgs a, int kv_dtype, int head_dim, int64_t rows, hipStream_t st) {
+  cap_series(&a.mod, a.scale_log2);
   if (kv_dtype == PKV_F16) return launch<PKV_F16, false>(a, head_dim, rows, st);
   return a.v16 ? launch<PKV_BF16, true>(a, head_dim, rows, st)
                : launch<PKV_BF16, false>(a, head_dim, rows, st);
