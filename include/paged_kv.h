@@ -378,7 +378,8 @@ int pkv_paged_prefill_rows(void* out, int out_dtype, int64_t out_stride_tok, int
 /*
  * Attention with modified scores (no counterpart in the reference, whose models cap no score and
  * mask causally only). The arguments after num_rows of the two calls below:
- *   softcap (0: none; else 1e-30 .. 1e30): s = softcap * tanh(scale * q . k / softcap);
+ *   softcap (0: none; else 1e-30 .. 1000): s = softcap * tanh(scale * q . k / softcap), off by some
+ *     5e-7 of softcap with 16-bit caches (hence its bound), by fp32 rounding of s with fp32 ones;
  *   alibi_slopes (fp32 [num_heads], or NULL): s -= alibi_slopes[h] * |query's position - key's|,
  *     after the cap; a decode query sits at context_lens[b] - 1, query i of a chunk of q_c tokens
  *     at n_c - q_c + i. Slopes are finite;

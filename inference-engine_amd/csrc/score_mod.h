@@ -55,11 +55,11 @@ __device__ __forceinline__ float biased(float d, float slope2, int far) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The entry points' score arguments, checked. softcap 0: no cap. c1 and c2 stay finite and away
-// from zero for every cap of fp32's normal range but its ends.
+// The entry points' score arguments, checked. softcap 0: no cap. Its upper bound keeps the error of
+// the 16-bit kernels' cap, some 2^-21 of it, below that of their weights.
 inline int score_mod(ScoreMod* m, float softcap, const float* slopes, const int32_t* ranges,
                      int64_t range_stride) {
-  if (!(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f))) return PKV_E_SHAPE;
+  if (!(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1000.f))) return PKV_E_SHAPE;
   if (ranges && range_stride < 0) return PKV_E_SHAPE;
   *m = {softcap > 0.f ? 2.f / softcap : 0.f, softcap * kLog2e, slopes, ranges, range_stride, {}, -1.f};
   return 0;
@@ -69,14 +69,14 @@ inline int score_mod(ScoreMod* m, float softcap, const float* slopes, const int3
 // x = scale_log2 s / c2, c2 tanh(x) = s (scale_log2 + s^2 (series[0] + s^2 series[1])). The coefficients
 // are the minimax ones of tanh(x) - x over [0, 0.3] (a linear program over 4,001 points): off by at most
 // 3.0e-07, relative 2.0e-06. series_max = -1 (no score) without a cap and where the coefficients could
-// overflow.
+// over- or underflow.
 inline void cap_series(ScoreMod* m, float scale_log2) {
   const double f = (double)scale_log2 / m->c2, co[2] = {-0.33312109, 0.12640677};
   m->series_max = -1.f;
   if (m->c2 == 0.f || !(f <= 1e4)) return;
   double g = scale_log2;
   for (int i = 0; i < 2; ++i) m->series[i] = (float)(co[i] * (g *= f * f));
-  m->series_max = (float)(0.3 / f);
+  if (m->series[1] >= 1e-37f) m->series_max = (float)(0.3 / f);  // 0 would take -inf to NaN
 }
 
 // A tile's raw scores s = q . k (RT row tiles of NB 16-key blocks, lane values [t][beta][r] =

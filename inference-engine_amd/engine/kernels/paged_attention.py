@@ -386,8 +386,8 @@ def paged_decode_attention(
     ``prefix_groups``). Rows that no sequence names keep what they hold.
 
     Modified scores (not with ``prefix_groups``; the reference has none):
-    ``softcap``: scores become ``softcap * tanh(score / softcap)``. ``alibi_slopes`` (float32
-    [nh], finite): then ``alibi_slopes[h] * (distance in tokens from the query to the key)`` is
+    ``softcap`` (at most 1000): scores become ``softcap * tanh(score / softcap)``, to within some
+    5e-7 of ``softcap`` with 16-bit caches. ``alibi_slopes`` (float32 [nh], finite): then ``alibi_slopes[h] * (distance in tokens from the query to the key)`` is
     taken off. ``key_ranges`` (int32 [rows of q, 2]): the query in row r of q sees the keys
     ``key_ranges[r, 0] <= p < key_ranges[r, 1]`` of its context and no others (a sliding window;
     ``step_key_ranges`` builds them); a range without keys gives 0, and what lies outside a range
@@ -490,8 +490,9 @@ def _score_mod(what: str, dev: torch.device, q: torch.Tensor, queries: int,
         return None
     nh = q.shape[1]
     cap = 0.0 if softcap is None else float(softcap)
-    if cap != 0.0 and not 1e-30 <= cap <= 1e30:
-        raise ValueError(f"{what}: softcap {softcap} must be positive and finite (0 or None: no cap)")
+    if cap != 0.0 and not 1e-30 <= cap <= 1000.0:
+        raise ValueError(f"{what}: softcap {softcap} must be positive and at most 1000 (0 or None: "
+                         "no cap)")  # fmt: skip
     for name, x in (("alibi_slopes", alibi_slopes), ("key_ranges", key_ranges), ("lse", lse)):
         if x is not None and x.device != dev:
             raise ValueError(f"{what}: {name} must be on {dev}, got {x.device}")
