@@ -840,8 +840,8 @@ def paged_attention_weights(
     ``evict_tokens`` chooses by). No counterpart in the reference, which evicts no token.
 
     weights: float32 [R, >= W * block_size], unit stride along positions; sequence c's is row
-    ``weight_rows[c]`` (int64 [C]; None: c; a row outside [0, R): the sequence is skipped; distinct
-    rows). q, k_cache, block_tables [C, W], context_lens [C], block_size, cu_seqlens_q [C + 1] and
+    ``weight_rows[c]`` (int64 [C]; None: c; a row outside [0, R): the sequence is skipped; the others
+    distinct, which the debug checks look at). q, k_cache, block_tables [C, W], context_lens [C], block_size, cu_seqlens_q [C + 1] and
     max_query_len as in ``paged_prefill_attention`` (cu_seqlens_q None: one query per sequence, as
     in ``paged_decode_attention``); a prompt's chunk can give its last queries alone (they are the
     last tokens of its context). lse: float32 [T, nh], contiguous, from the attention call over the
@@ -948,6 +948,10 @@ def _check_weight_rows(what: str, weight_rows: torch.Tensor | None, batch: int, 
     elif weight_rows.dtype != torch.int64 or weight_rows.shape != (batch,) or \
             not weight_rows.is_contiguous():  # fmt: skip
         raise ValueError(f"{what}: weight_rows must be a contiguous int64 [{batch}] tensor")
+    elif _native.debug_checks():
+        used = weight_rows[(weight_rows >= 0) & (weight_rows < rows)]
+        if used.unique().numel() != used.numel():
+            raise IndexError(f"{what}: two sequences with one row of weights")
 
 
 # Largest workspace paged_prefill_attention allocates by itself for the fp16 V copy.
