@@ -250,11 +250,15 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_no_guard = contextlib.nullcontext()
+
+
 def device_guard(device: torch.device):
     """``device`` as the current one while the library is called (it asks the current device for
     its CUs); nothing where it is already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index is None or device.index == _current_device():
+        return _no_guard
     return torch.cuda.device(device)
 
 

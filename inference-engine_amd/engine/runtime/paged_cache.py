@@ -9,12 +9,14 @@ decode kernel streams and what ``copy_blocks`` moves.
 
 from __future__ import annotations
 
+import functools
 from collections.abc import Sequence
 from dataclasses import dataclass
 
 import torch
 
 from engine.kernels import _native
+from engine.kernels.paged_attention import _check_weight_rows
 
 
 @dataclass(frozen=True)
@@ -222,8 +224,6 @@ def evict_tokens(
                          "unit stride along positions")  # fmt: skip
     if layers > 1 and weights.stride(0) < (weights.shape[1] - 1) * weights.stride(1) + weights.shape[2]:
         raise ValueError(f"{what}: layers of weights overlap")
-    from engine.kernels.paged_attention import _check_weight_rows
-
     _check_weight_rows(what, weight_rows, b, weights.shape[1], weights.stride(1), weights.shape[2])
     if out is None:
         out = torch.empty_like(context_lens)
@@ -238,9 +238,7 @@ def evict_tokens(
         _check_own_blocks(what, block_tables, context_lens, block_size, keep, weight_rows,
                           weights.shape[1])  # fmt: skip
     lib = _native.lib()
-    need = lib.pkv_evict_workspace_bytes(layers, b, width, block_size, keep)
-    if need < 0:
-        _native.check(need, what)
+    need = evict_workspace_bytes(layers, b, width, block_size, keep)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     elif workspace.dtype != torch.uint8 or workspace.numel() < need or not workspace.is_contiguous():
@@ -258,6 +256,7 @@ def evict_tokens(
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def evict_workspace_bytes(layers: int, batch: int, max_blocks: int, block_size: int, keep: int) -> int:
     """Scratch of one ``evict_tokens`` call of these sizes, e.g. to allocate it outside a capture."""
     n = _native.lib().pkv_evict_workspace_bytes(layers, batch, max_blocks, block_size,
