@@ -157,18 +157,22 @@ template <int DT, int HD, int RT> struct WRows {
       lse[t][0] = x.x, lse[t][1] = x.y, lse[t][2] = x.z, lse[t][3] = x.w;
     }
   }
+  // The same where every row sees every key of the tile and scores are as they are.
+  __device__ __forceinline__ float plain_weight(const WeightsArgs& a, const f32x4 (&s)[RT]) const {
+    float acc[2] = {0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[r & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.scale_log2, -lse[t][r]));
+    return acc[0] + acc[1];
+  }
   // The weights of key kt + col over this lane's rows, from the tile's scores. here: the key exists.
   __device__ __forceinline__ float weight(const WeightsArgs& a, const RowLds<RT>& l, const f32x4 (&s)[RT],
                                           int kt, bool here, bool plain) const {
+    if (plain && lo_max <= kt && kt + 16 <= hi_min && __ballot(here) == ~0ull)  // uniform
+      return plain_weight(a, s);
     float acc[2] = {0.f, 0.f};
-    if (plain && lo_max <= kt && kt + 16 <= hi_min && __ballot(here) == ~0ull) {  // uniform
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          acc[r & 1] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], a.scale_log2, -lse[t][r]));
-      return acc[0] + acc[1];
-    }
     const int lane = threadIdx.x & (kWave - 1), key = kt + (lane & 15), grp = lane >> 4;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -185,6 +189,16 @@ template <int DT, int HD, int RT> struct WRows {
     return acc[0] + acc[1];
   }
 };
+// x[l] + x[l ^ 32] in the lower 32 lanes, y's in the upper ones; likewise for rows of 16 lanes (x's
+// in the even rows, y's in the odd ones).
+__device__ __forceinline__ float swap_add32(float x, float y) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float swap_add16(float x, float y) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
 // LDS that one wave wrote for itself may be read.
 __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -299,9 +313,12 @@ attention_weights_few_kernel(const WeightsArgs a) {
 // RT query rows each in registers and all walk over the span's keys, TK at a time through LDS (rows
 // padded by 16 bytes: the operand reads of 16 keys then cover all banks), the next tile's K on its
 // way under this one's scores. Each KV head's sums go to the workspace, and a second launch adds them
-// up in the order of the heads, with the decay. Bound by an exp2 per score. (With all KV heads in one
-// workgroup, no second launch, every workgroup read all queries, 512 KB for 64 keys, and waited for
-// them head by head: 8 prompts of 64 queries over 2,000-8,000 tokens, 32 / 8 heads, hd 128: 76 us.)
+// up in the order of the heads, with the decay. Bound by vector instructions: an exp2, a
+// multiply-add and an add per score. 8 prompts of 64 queries over 2,000-8,000 tokens, 32 / 8 heads, hd
+// 128, bf16: 41 us and 4 for the second launch; 46 before tiles that every row sees whole had a path
+// without a branch per 16 keys. (With all KV heads in one workgroup, no second launch, every workgroup
+// read all queries, 512 KB for 64 keys, and waited for them head by head: 76 us. With runs of tiles of
+// equal length over chunks and heads, one per workgroup that the card holds: as fast, and spilled.)
 constexpr int kManyWaves = 8, kManySpan = 2048;
 template <int DT, int HD> struct MShape {
   static constexpr int NF = WShape<DT, HD>::NF;
@@ -339,11 +356,13 @@ attention_weights_many_kernel(const WeightsArgs a) {
   if (kg >= k.n || k.wrow < 0 || k.wrow >= a.w_num) return;  // uniform
   const int k_end = min(k.n, kg + a.span);
   // The span's slots, -1 past the context or outside the pool.
+  bool bad = false;  // a key of the span without a slot
   for (int i = tid; i < a.span; i += THREADS) {
     const int p = kg + i, blk = a.bs_shift >= 0 ? p >> a.bs_shift : p / a.bs;
     const int id = p < k_end ? a.tables[(int64_t)c * a.table_stride + blk] : -1;
     const int64_t sl = (int64_t)id * a.bs + (p - blk * a.bs);
     slots[i] = id >= 0 && sl < a.num_slots ? (int)sl : -1;  // num_slots < 2^31 (launch)
+    bad = bad || (p < k_end && slots[i] < 0);
   }
   float* const out = a.ws + ((int64_t)c * a.nkv + kvh) * cap;
   const bool dims = HD >= 4 * VEC || grp * VEC < HD;
@@ -380,7 +399,7 @@ attention_weights_many_kernel(const WeightsArgs a) {
     const bool has = row0 < k.nrows;  // uniform per wave
     WRows<DT, HD, RT> rows;
     rows.first = 0x7FFFFFFF, rows.last = 0;
-    __syncthreads();  // the slots; the row block before is done with its LDS
+    const bool holes = __syncthreads_or(bad);  // the slots; the row block before is done with its LDS
     if (has) {
       rows.rows(a, k, kvh, row0, row_lds[wave]);
       rows.load_q(a, k, kvh, row0);
@@ -415,25 +434,43 @@ attention_weights_many_kernel(const WeightsArgs a) {
       if (more) load_k(k0 + TK, st);
       if (k0 > t_beg) put(k0 - TK, buf ^ 1, rb > 0);
       float v[NT];
+      if (has && plain && !holes && rows.lo_max <= k0 && k0 + TK <= min(rows.hi_min, k_end)) {  // uniform
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        v[t] = 0.f;
-        const int kt = k0 + 16 * t;
-        if (!has || kt >= rows.last || kt + 16 <= rows.first) continue;  // uniform
-        const bool here = slots[min(kt - kg + col, a.span - 1)] >= 0;
-        u32x4 kf[NF];
+        for (int t = 0; t < NT; t += 2) {  // two blocks' chains of products at a time
+          f32x4 s[2][RT];
 #pragma unroll
-        for (int m = 0; m < NF; ++m) kf[m] = kv[buf][(16 * t + col) * LDW + (dims ? 4 * m + grp : 0)];
-        f32x4 s[RT];
+          for (int u = 0; u < 2; ++u) {
+            u32x4 kf[NF];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) s[i] = score_tile<DT, HD>(rows.q[i], kf);
-        v[t] = rows.weight(a, row_lds[wave], s, kt, here, plain);
+            for (int m = 0; m < NF; ++m) kf[m] = kv[buf][(16 * (t + u) + col) * LDW + (dims ? 4 * m + grp : 0)];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) s[u][i] = score_tile<DT, HD>(rows.q[i], kf);
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) v[t + u] = rows.plain_weight(a, s[u]);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          v[t] = 0.f;
+          const int kt = k0 + 16 * t;
+          if (!has || kt >= rows.last || kt + 16 <= rows.first) continue;  // uniform
+          const bool here = slots[min(kt - kg + col, a.span - 1)] >= 0;
+          u32x4 kf[NF];
+#pragma unroll
+          for (int m = 0; m < NF; ++m) kf[m] = kv[buf][(16 * t + col) * LDW + (dims ? 4 * m + grp : 0)];
+          f32x4 s[RT];
+#pragma unroll
+          for (int i = 0; i < RT; ++i) s[i] = score_tile<DT, HD>(rows.q[i], kf);
+          v[t] = rows.weight(a, row_lds[wave], s, kt, here, plain);
+        }
       }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float x = rows_sum(v[t]);
-        if (grp == t % 4) part[buf][wave][16 * t + col] = x;
-      }
+      // Lane (col, grp) gets the sum over the rows of lanes for key 16 grp + col (two blocks: 16
+      // (grp / 2) + col): each swap brings two blocks' halves side by side.
+      float x = swap_add32(v[0], v[NT / 2]);
+      if constexpr (NT == 4) x = swap_add16(x, swap_add32(v[1], v[3]));
+      else x = swap_add16(x, x);
+      if (NT == 4 || grp % 2 == 0) part[buf][wave][16 * (NT == 4 ? grp : grp / 2) + col] = x;
       if (more) store_k(buf ^ 1, st);
     }
     __syncthreads();
@@ -469,7 +506,8 @@ template <int DT, int HD> hipError_t launch_weights_hd(WeightsArgs a, int64_t ro
     const int least = 16 * (kFewWaves / a.tw) > 64 ? 16 * (kFewWaves / a.tw) : 64;
     while (a.span > least && a.n_chunks * ((cap + a.span - 1) / a.span) < 512) a.span /= 2;
   } else {
-    // Keys per workgroup: a multiple of the tiles', about two workgroups per CU and half as many again.
+    // Keys per workgroup: a multiple of the tiles', about two workgroups per CU and half as many again
+    // (the prompts above: 46 us with 512 keys or 1,024, 49 with 256).
     a.span = kManySpan;
     while (a.span > 128 && a.n_chunks * a.nkv * ((cap + a.span - 1) / a.span) < 768) a.span /= 2;
   }

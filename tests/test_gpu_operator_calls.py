@@ -36,6 +36,21 @@ def test_weights_of_more_rows_than_a_workgroup_holds(shape, mods):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("dtype,hd", [(BF16, 128), (FP16, 64), (FP32, 256)])
+def test_weights_of_many_rows_over_bad_blocks(dtype, hd):
+    """A block id outside the pool holds no key, in tiles that every row sees whole as in others."""
+    s = Step(dtype, 4, 1, hd, 16, [300], [20], seed=33)
+    lse = attention64(s)[1].float()
+    old = torch.rand(1, s.tables.shape[1] * 16, generator=torch.Generator().manual_seed(3))
+    want = weights64(s, old, 1.0, lse)
+    for block, bad in ((2, -1), (9, 1 << 30), (18, -7)):
+        want[0, 16 * block : 16 * block + 16] = old[0, 16 * block : 16 * block + 16].double()
+        s.tables[0, block] = bad
+    got = run(s, old.cuda(), (None, None, None), lse).cpu()
+    err = (got.double() - want).abs()
+    assert bool((err <= bound(s, want, old, 1.0, (None, None, None))).all())
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1], [40, 3, 9]])
 def test_weights_captured(new):
     """One graph, other lengths, queries, normalisers and weights at every replay."""
