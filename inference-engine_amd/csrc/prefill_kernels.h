@@ -359,13 +359,18 @@ struct KeyBounds {
 };
 __device__ __forceinline__ KeyBounds key_bounds(int beg, int end, int lo_m, int hi_m, int wave) {
   __shared__ int bounds[8][4];
-#pragma unroll
-  for (int off = 1; off < 16; off <<= 1) {  // the four rows of lanes hold the same query rows
-    beg = min(beg, __shfl_xor(beg, off));
-    end = max(end, __shfl_xor(end, off));
-    lo_m = max(lo_m, __shfl_xor(lo_m, off));
-    hi_m = min(hi_m, __shfl_xor(hi_m, off));
-  }
+  // Over a row of 16 lanes (the four rows hold the same query rows).
+  auto step = [&](auto ctrl) __attribute__((always_inline)) {
+    constexpr int C = decltype(ctrl)::value;
+    beg = min(beg, __builtin_amdgcn_update_dpp(0, beg, C, 0xF, 0xF, false));
+    end = max(end, __builtin_amdgcn_update_dpp(0, end, C, 0xF, 0xF, false));
+    lo_m = max(lo_m, __builtin_amdgcn_update_dpp(0, lo_m, C, 0xF, 0xF, false));
+    hi_m = min(hi_m, __builtin_amdgcn_update_dpp(0, hi_m, C, 0xF, 0xF, false));
+  };
+  step(std::integral_constant<int, kQuadXor1>{});
+  step(std::integral_constant<int, kQuadXor2>{});
+  step(std::integral_constant<int, kRowHalfMirror>{});
+  step(std::integral_constant<int, kRowMirror>{});
   if ((threadIdx.x & (kWave - 1)) == 0) {
     bounds[wave][0] = beg;
     bounds[wave][1] = end;
@@ -526,6 +531,21 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
   int row_out[RT];  // the row of out
   bool row_ok[RT];
   u32x4 qf[RT][KS];
+  [[maybe_unused]] int range[RT][2];  // MOD: the row's keys; loaded before the queries, which are needed later
+  if constexpr (MOD) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int rho = rho0 + 16 * RT * wave + 16 * t + col;
+      int64_t row = q0 + (rho < nrows ? rho : 0) / G;
+      if (a.rows) row = max(token_row(a, row), (int64_t)0);
+      range[t][0] = range[t][1] = 0;
+      if (a.mod.ranges) {
+        const int32_t* r = a.mod.ranges + row * a.mod.range_stride;
+        range[t][0] = r[0];
+        range[t][1] = r[1];
+      }
+    }
+  }
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int rho = rho0 + 16 * RT * wave + 16 * t + col;
@@ -586,8 +606,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
       for (int t = 0; t < RT; ++t) {
         mlast[t] = -1;  // no query, or no key: nothing
         if (row_ok[t]) {
-          const int32_t* r = a.mod.ranges + (int64_t)row_out[t] * a.mod.range_stride;
-          const int lo = max(r[0], 0), hi = min(r[1], n);
+          const int lo = max(range[t][0], 0), hi = min(range[t][1], n);
           hi_m = min(hi_m, lo < hi ? hi : 0);
           if (lo < hi) {
             mfirst[t] = lo;
