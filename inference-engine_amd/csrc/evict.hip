@@ -217,23 +217,26 @@ evict_select_kernel(const EvictArgs a) {
 // ---------------------------------------------------------------------------------
 // Move: kept token i goes from its slot to token i's, for every i from the first gap on.
 //
-// A token moves down (from >= to), and moves go up in i, so in one wave that reads a batch of
-// tokens before it writes them, and takes the batches in order, nothing is overwritten unread: a
+// A token moves down (from >= to), and moves go up in i, so where a batch of tokens is read before any
+// of it is written, and the batches follow each other in order, nothing is overwritten unread: a
 // later batch's sources lie at or past every earlier batch's destinations. The bytes of a row are
-// independent, so a wave takes a slice of SLICE bytes of every row of one (layer, sequence, K or V)
-// and needs no other wave. The next batch's rows are on their way while this one's are written.
-// Bound by HBM, every row read and written once.
+// independent, so a workgroup takes a slice of SLICE bytes of every row of one (layer, sequence, K
+// or V) and needs no other workgroup; its W waves take shares of a batch, with one barrier between
+// its reads and its writes (W = 1: a workgroup of four waves with a slice each). The next batch's rows
+// are on their way while this one's are written. Bound by HBM, every row read and written once.
+// Figures at the launch.
 // ---------------------------------------------------------------------------------
 
-template <int SLICE>
-__global__ void __launch_bounds__(256)
+template <int SLICE, int W>
+__global__ void __launch_bounds__(W > 1 ? W * kWave : 4 * kWave)
 evict_move_kernel(const EvictArgs a, int slices) {
   constexpr int LPR = SLICE / 16;      // lanes per row
   constexpr int RPL = kWave / LPR;     // rows per load
   constexpr int U = 8;                 // loads per batch
-  constexpr int BATCH = RPL * U;
+  constexpr int BATCH = RPL * U * W;
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t job = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;  // slices innermost
+  const int wave = threadIdx.x / kWave;
+  const int64_t job = W > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;  // slices innermost
   const int64_t per = 2 * (int64_t)slices;
   const int64_t seq = job / per;
   if (seq >= (int64_t)a.layers * a.batch) return;
@@ -247,7 +250,7 @@ evict_move_kernel(const EvictArgs a, int slices) {
   char* pool = (part / slices ? a.v : a.k) + (seq / a.batch) * a.layer_bytes + at;
   const int32_t* from = a.from + seq * a.keep_stride;
   const int32_t* trow = a.tables + (seq % a.batch) * a.table_stride;
-  const int r = lane / LPR;
+  const int r = lane / LPR + (W > 1 ? wave * (RPL * U) : 0);  // this lane's first row of a batch
 
   // Loads go out without conditions (a token past the end reads the last one's, a slot outside the
   // pool and a lane past the row slot 0), so that the wait for one batch does not wait for the next;
@@ -278,10 +281,12 @@ evict_move_kernel(const EvictArgs a, int slices) {
     load_moves(i + 2 * BATCH, after);
     load_rows(next, nx);
     // Every row of this batch is in registers before any of it is overwritten: one statement that
-    // takes them all.
+    // takes a wave's all, and a barrier without a fence (which would wait for the next batch's rows).
     static_assert(U == 8, "the rows of a batch below");
     __asm__ volatile("" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]),
                           "+v"(x[6]), "+v"(x[7]) : : "memory");
+    if constexpr (W > 1) __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" : : : "memory");
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int p = i + u * RPL + r;
@@ -296,11 +301,12 @@ evict_move_kernel(const EvictArgs a, int slices) {
   }
 }
 
-template <int SLICE> int launch_move(const EvictArgs& a, int64_t seqs, hipStream_t st) {
-  const int64_t slices = (a.row_bytes + SLICE - 1) / SLICE;
-  const int64_t wgs = (seqs * 2 * slices + 3) / 4;
+template <int SLICE, int W> int launch_move(const EvictArgs& a, int64_t seqs, hipStream_t st) {
+  const int64_t slices = (a.row_bytes + SLICE - 1) / SLICE, jobs = seqs * 2 * slices;
+  const int64_t wgs = W > 1 ? jobs : (jobs + 3) / 4;
   if (slices > (1 << 20) || wgs >= ((int64_t)1 << 24)) return PKV_E_SHAPE;
-  hipLaunchKernelGGL(evict_move_kernel<SLICE>, dim3((unsigned)wgs), dim3(256), 0, st, a, (int)slices);
+  hipLaunchKernelGGL((evict_move_kernel<SLICE, W>), dim3((unsigned)wgs), dim3(W > 1 ? W * kWave : 4 * kWave), 0,
+                     st, a, (int)slices);
   return (int)hipGetLastError();
 }
 
@@ -384,15 +390,16 @@ int pkv_evict(void* k_pool, void* v_pool, int64_t layer_stride_bytes, int32_t la
   else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || cap <= keep) return (int)e;
-  // The widest slices that still make 16 waves per CU: 256 bytes keep a row's bytes together in
-  // memory (16 layers, 32 sequences down to 1,000 tokens of 1 KB rows, weights and all: 414 us, with 64
-  // bytes 552); where not even 64 make four per CU, 32 (16 layers, one sequence of 2,112 tokens down to
-  // 2,048: 35 us, with 64 bytes 38, with 256 143).
-  const int64_t pairs = seqs * 2;
-  if (pairs * ((row_bytes + 255) / 256) >= 4096) return launch_move<256>(a, seqs, st);
-  if (pairs * ((row_bytes + 127) / 128) >= 4096) return launch_move<128>(a, seqs, st);
-  if (pairs * ((row_bytes + 63) / 64) >= 1024) return launch_move<64>(a, seqs, st);
-  return launch_move<32>(a, seqs, st);
+  // Slices of 256 bytes keep a row's bytes together in memory, of 128 make twice the workgroups; the
+  // wide ones where they are more than one per CU. Whole calls, rows of 1 KB, wide and narrow: 16
+  // layers, 4 sequences of 8,192 tokens down to 8,000 448 and 479 us; one sequence of 2,112 down to 2,048
+  // 34 and 31, of 32,768 down to 30,000 532 and 508 (single waves with narrower slices, down to 32
+  // bytes: 615, 37, 743). A wave per slice where that makes 16 per CU: 32 sequences of 700-4,096 down
+  // to 1,000 412 us, with 8 waves 427.
+  const int64_t wide = seqs * 2 * ((row_bytes + 255) / 256);
+  if (wide >= 4096) return launch_move<256, 1>(a, seqs, st);
+  if (wide > 256) return launch_move<256, 8>(a, seqs, st);
+  return launch_move<128, 8>(a, seqs, st);
 }
 
 }  // extern "C"

@@ -58,6 +58,36 @@ def test_evict_lengths(n):
     check(s, k, v, w, n - 1, n - 1)
 
 
+@pytest.mark.parametrize("layers,batch,n,keep", [(2, 3, 1500, 1200), (4, 20, 700, 650), (16, 34, 300, 120)])
+def test_evict_wide_rows(layers, batch, n, keep):
+    """Rows of 1 KB, few and many sequences (each width of the move pass), batches of rows that
+    overlap their own destinations."""
+    g = torch.Generator().manual_seed(batch)
+    ctx = [n - 7 * i % 90 for i in range(batch)]
+    width = -(-n // 16)
+    tables = torch.randperm(batch * width, generator=g).view(batch, width).int()
+    k = torch.randint(-(2**15), 2**15, (layers, batch * width * 16, 8, 64), generator=g).to(torch.bfloat16)
+    v = torch.randint(-(2**15), 2**15, k.shape, generator=g).to(torch.bfloat16)
+    w = torch.rand(layers, batch, width * 16, generator=g, dtype=torch.float64).float()
+    slots = (tables.long()[..., None] * 16 + torch.arange(16)).flatten(1)
+    want_k, want_v, want_w = k.clone(), v.clone(), w.clone()
+    for layer in range(layers):
+        for b, m in enumerate(ctx):
+            if m <= keep:
+                continue
+            old = m - 32
+            heavy = torch.sort(w[layer, b, :old], descending=True, stable=True).indices[: keep - 32]
+            kept = torch.cat([heavy.sort().values, torch.arange(old, m)])
+            src, dst = slots[b, kept], slots[b, :keep]
+            want_k[layer, dst], want_v[layer, dst] = k[layer, src], v[layer, src]
+            want_w[layer, b, :keep], want_w[layer, b, keep:m] = w[layer, b, kept], 0.0
+    gk, gv, gw = k.cuda(), v.cuda(), w.cuda()
+    out = evict_tokens(gk, gv, gw, tables.cuda(), torch.tensor(ctx, dtype=torch.int32).cuda(), 16, keep, 32)
+    assert out.tolist() == [min(m, keep) for m in ctx]
+    assert torch.equal(gk.cpu(), want_k) and torch.equal(gv.cpu(), want_v)
+    assert torch.equal(gw.cpu(), want_w)
+
+
 def test_evict_ties_and_special_weights():
     """Equal weights, zeros of both signs, negatives, infinities and NaN: the lowest positions of
     what is equal stay, a NaN goes first."""
