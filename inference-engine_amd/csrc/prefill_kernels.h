@@ -489,8 +489,8 @@ template <int HD> struct PrefillLds {
 //   kModCap: a cap, no bias. Scores stay raw until the exponent, where the cap costs 3 multiply-adds
 //     each (a tile with a score past 0.3 of the cap: the exact form, an exp2 and a reciprocal).
 //   kModBias: a bias, no cap. It is what Q.K^T starts its sums from, so the softmax sees it as part of
-//     the raw score. Taken against the row's nearest key, whose bias the normaliser gets back: its
-//     rounding then matters only to weights that it makes small.
+//     the raw score. Taken against the row's nearest key (a negative slope: the farthest), whose bias
+//     the normaliser gets back: its rounding then matters only to weights that it makes small.
 //   kModAny: both, either or none.
 // One prompt of 6,011 tokens, 32 / 8 heads, head_dim 128, bf16, on a day when the plain kernel took
 // 303 us with the copy of V: ranges 314, cap 353 (412 where every tile takes the exact form), bias
@@ -852,7 +852,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
     if constexpr (MOD) return j * KT < lo_max || (j + 1) * KT > hi_min;
     else return j >= j_mask;
   };
-  // The bias of a row's head, in log2 units (kModAny) or raw ones with the nearest key's (kModBias).
+  // The bias of a row's head, in log2 units (kModAny) or raw ones with its least one's (kModBias).
   [[maybe_unused]] float slope[RT], nearest[RT];
   if constexpr (MOD >= kModBias) {
 #pragma unroll
@@ -862,7 +862,8 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a, const Prefill
       if constexpr (MOD == kModBias) {
         slope[t] /= a.scale_log2;
         const int pos = base_pos + row_tok[t];
-        nearest[t] = slope[t] * (float)max(max(pos - mlast[t], mfirst[t] - pos), 0);
+        const int before = pos - mfirst[t], after = mlast[t] - pos;
+        nearest[t] = slope[t] * (float)(slope[t] < 0.f ? max(abs(before), abs(after)) : max(max(-before, -after), 0));
       }
     }
   }

@@ -14,8 +14,10 @@ template <int DT, int HD, bool V16> hipError_t launch_hd(PrefillArgs a, int64_t 
   const int64_t items = (int64_t)a.row_blocks * a.nkv * a.n_chunks;
   if (items > 0x7FFFFFFF) return hipErrorInvalidValue;
   const dim3 grid((unsigned)items), block(512);
-  // Block sizes that are no power of two have the general kernel only.
-  const int mod = a.bs_shift < 0 ? 0 : a.mod.slopes ? (a.mod.c2 != 0.f ? kModAny : kModBias)
+  // Block sizes that are no power of two have the general kernel only; a bias in units of tiny scales
+  // could overflow.
+  const bool bias_only = a.mod.c2 == 0.f && a.scale_log2 >= 1e-12f;
+  const int mod = a.bs_shift < 0 ? 0 : a.mod.slopes ? (bias_only ? kModBias : kModAny)
                                                     : (a.mod.c2 != 0.f ? kModCap : kModRanges);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a); };
   switch (mod) {

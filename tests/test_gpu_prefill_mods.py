@@ -50,10 +50,12 @@ def test_cap_of_small_and_large_scores(shape, cap, distance):
     check(s, prefill(s, how, lse=lse), lse, how, True)
 
 
+@pytest.mark.parametrize("sign", [1, -1])
 @pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[1], SHAPES[5]], ids=str)
-def test_bias_of_far_keys(shape):
+def test_bias_of_far_keys(shape, sign):
     """Rows that see only keys far behind them, or ahead of them, or one key: the bias common to a
-    row's keys does not cost the others their bits, and the normaliser holds it."""
+    row's keys does not cost the others their bits, and the normaliser holds it. A negative slope
+    favours the far ones."""
     dtype, nh, nkv, hd, bs, _ = shape
     ctx, new = [1500, 700], [30, 40]
     s = Step(dtype, nh, nkv, hd, bs, ctx, new, seed=23)
@@ -61,7 +63,7 @@ def test_bias_of_far_keys(shape):
     for j, (i, p) in enumerate(s.positions()):
         rows.append([[0, 90], [p - 3, p - 2], [p + 1, p + 9], [max(0, p - 700), p + 1], [40, 41]][(j + i) % 5])
     ranges = torch.tensor(rows, dtype=torch.int32)
-    how = (None, slopes_of(nh), ranges)
+    how = (None, sign * slopes_of(nh), ranges)
     lse = torch.empty(s.q.shape[:2], device="cuda")
     check(s, prefill(s, how, lse=lse), lse, how, True)
 
